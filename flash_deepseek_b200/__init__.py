@@ -8,6 +8,9 @@ engine's own seams (JohnnyNg6/flash_deepseek, infer.m):
     MoE.experts_forward  metal_moe_forward()    infer.m:1604-1700
     MoE.shared_forward   shared_expert_worker() infer.m:1099-1114
     MoE.forward          MoE half of layer_forward, infer.m:1878-1922
+    MoE.rope_device      apply_rope_q / _k()    infer.m:628-656
+    MoE.kv_write_device, MoE.kv_read_device, MoE.mla_attention_device
+                         cache and attention of mla_forward(), infer.m:665-903
     dequantize_row_q4_K / dequantize_row_q6_K   quant.h:11-12
 
 Host arrays are numpy; device buffers may be given as integer pointers or as
@@ -22,7 +25,7 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from ._lib import MoeConfigC, load as load_library
+from ._lib import KVBatchC, KVCacheC, MlaQueryC, MoeConfigC, RopeConfigC, load as load_library
 
 TYPE_F32 = 0  # GGML_TYPE_F32
 TYPE_F16 = 1  # GGML_TYPE_F16
@@ -30,6 +33,8 @@ TYPE_Q4_K = 12  # GGML_TYPE_Q4_K (gguf.h:59)
 TYPE_Q6_K = 14  # GGML_TYPE_Q6_K (gguf.h:61)
 TYPE_BF16 = 30  # GGML_TYPE_BF16
 QK_K = 256
+KV_F16, KV_BF16, KV_FP8_F16, KV_FP8_BF16 = 1, 30, 101, 130  # formats of the latent cache's rows
+KV_ROPE = 64  # rotary values of a cache row
 BLOCK_BYTES = {TYPE_Q4_K: 144, TYPE_Q6_K: 210}
 
 
@@ -73,6 +78,37 @@ def _ptr(a):
 def _f32(a, shape=None):
     a = np.ascontiguousarray(a, dtype=np.float32)
     return a if shape is None else a.reshape(shape)
+
+
+class RopeConfig:
+    """Rotary frequencies (moe_rope_config; DeepSeek-V3's YaRN by default)."""
+
+    def __init__(self, dim: int = KV_ROPE, half_layout: bool = False, theta: float = 10000.0, scale: float = 40.0,
+                 orig_ctx: float = 4096.0, beta_fast: float = 32.0, beta_slow: float = 1.0, mscale: float = 1.0):
+        self.c = RopeConfigC(dim, int(half_layout), theta, scale, orig_ctx, beta_fast, beta_slow, mscale)
+
+
+class KVCache:
+    """A paged latent cache in device memory (moe_kv_cache): n_pages pages of
+    page_size rows of kv_row_bytes(fmt, latent) bytes at `data`, which is kept
+    alive by this object."""
+
+    def __init__(self, data, fmt: int, latent: int, page_size: int, n_pages: int):
+        self.data = data
+        self.c = KVCacheC(_ptr(data), fmt, latent, page_size, n_pages)
+
+
+class KVBatch:
+    """The rows of a call (moe_kv_batch); device int32 buffers, kept alive by
+    this object."""
+
+    def __init__(self, n_seqs: int, n_tokens: int, q_start, ctx_len, pages, pages_per_seq: int):
+        self.bufs = (q_start, ctx_len, pages)
+        self.c = KVBatchC(n_seqs, n_tokens, _ptr(q_start), _ptr(ctx_len), _ptr(pages), pages_per_seq)
+
+
+def kv_row_bytes(fmt: int, latent: int) -> int:
+    return int(load_library().moe_kv_row_bytes(fmt, latent))
 
 
 def row_bytes(qtype: int, cols: int) -> int:
@@ -304,6 +340,37 @@ class MoE:
         self._check(self.lib.moe_sample_device(self.ctx, _ptr(d_logits), n_tokens, vocab, temp, top_p, rng_state,
                                                _ptr(d_tokens), _ptr(stream)), "moe_sample_device")
 
+    # ----------------------------------------- MLA attention, latent cache
+    def rope_device(self, rope: RopeConfig, d_x, x_type: int, x_strides, d_y, y_type: int, y_strides, d_pos,
+                    n_tokens: int, n_heads: int, head_dim: int, offset: int = 0, stream=None):
+        """Strides: (token, head) in elements."""
+        self._check(self.lib.moe_rope_device(self.ctx, rope.c, _ptr(d_x), x_type, x_strides[0], x_strides[1],
+                                             _ptr(d_y), y_type, y_strides[0], y_strides[1], _ptr(d_pos), n_tokens,
+                                             n_heads, head_dim, offset, _ptr(stream)), "moe_rope_device")
+
+    def kv_write_device(self, kv: KVCache, batch: KVBatch, d_kv_a, kv_type: int, row_stride: int, d_norm_w=None,
+                        eps: float = 1e-6, rope: RopeConfig | None = None, d_pos=None, stream=None):
+        self._check(self.lib.moe_kv_write_device(self.ctx, kv.c, batch.c, _ptr(d_kv_a), kv_type, row_stride,
+                                                 _ptr(d_norm_w), eps, None if rope is None else rope.c, _ptr(d_pos),
+                                                 _ptr(stream)), "moe_kv_write_device")
+
+    def kv_read_device(self, kv: KVCache, batch: KVBatch, d_out, out_type: int, row_stride: int, stream=None):
+        self._check(self.lib.moe_kv_read_device(self.ctx, kv.c, batch.c, _ptr(d_out), out_type, row_stride,
+                                                _ptr(stream)), "moe_kv_read_device")
+
+    def mla_workspace_bytes(self, latent: int = 512) -> int:
+        return int(self.lib.moe_mla_workspace_bytes(self.ctx, latent))
+
+    def mla_attention_device(self, kv: KVCache, batch: KVBatch, q_latent, q_latent_strides, q_rope, q_rope_strides,
+                             n_heads: int, scale: float, out, out_strides, workspace, workspace_bytes: int, lse=None,
+                             tree=None, tree_words: int = 0, stream=None):
+        """Strides: (token, head) in elements."""
+        q = MlaQueryC(_ptr(q_latent), q_latent_strides[0], q_latent_strides[1], _ptr(q_rope), q_rope_strides[0],
+                      q_rope_strides[1], n_heads, scale, _ptr(tree), tree_words, _ptr(out), out_strides[0],
+                      out_strides[1], _ptr(lse))
+        self._check(self.lib.moe_mla_attention_device(self.ctx, kv.c, batch.c, q, _ptr(workspace), workspace_bytes,
+                                                      _ptr(stream)), "moe_mla_attention_device")
+
     # --------------------------------------------------------------- forward
     def forward(self, layer: int, h_post):
         """MoE block on host arrays: returns (out [T,H], idx [T,K], w [T,K])."""
@@ -402,5 +469,6 @@ def dequantize_row_q6_K(src, n: int) -> np.ndarray:
     return out
 
 
-__all__ = ["MoE", "MoeConfig", "MoeError", "TYPE_BF16", "TYPE_F16", "TYPE_F32", "TYPE_Q4_K", "TYPE_Q6_K", "dequantize_row_q4_K", "dequantize_row_q6_K",
-           "get_unique_id", "load_library", "row_bytes"]
+__all__ = ["KVBatch", "KVCache", "KV_BF16", "KV_F16", "KV_FP8_BF16", "KV_FP8_F16", "KV_ROPE", "MoE", "MoeConfig",
+           "MoeError", "RopeConfig", "TYPE_BF16", "TYPE_F16", "TYPE_F32", "TYPE_Q4_K", "TYPE_Q6_K", "dequantize_row_q4_K", "dequantize_row_q6_K",
+           "get_unique_id", "kv_row_bytes", "load_library", "row_bytes"]

@@ -18,6 +18,29 @@ class MoeConfigC(C.Structure):
                 ("n_layers", C.c_int), ("max_tokens", C.c_int)]
 
 
+class RopeConfigC(C.Structure):
+    _fields_ = [("dim", C.c_int), ("half_layout", C.c_int), ("theta", C.c_float), ("scale", C.c_float),
+                ("orig_ctx", C.c_float), ("beta_fast", C.c_float), ("beta_slow", C.c_float), ("mscale", C.c_float)]
+
+
+class KVCacheC(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("format", C.c_int), ("latent", C.c_int), ("page_size", C.c_int),
+                ("n_pages", C.c_int)]
+
+
+class KVBatchC(C.Structure):
+    _fields_ = [("n_seqs", C.c_int), ("n_tokens", C.c_int), ("q_start", C.c_void_p), ("ctx_len", C.c_void_p),
+                ("pages", C.c_void_p), ("pages_per_seq", C.c_int)]
+
+
+class MlaQueryC(C.Structure):
+    _fields_ = [("q_latent", C.c_void_p), ("q_latent_token_stride", C.c_int64), ("q_latent_head_stride", C.c_int64),
+                ("q_rope", C.c_void_p), ("q_rope_token_stride", C.c_int64), ("q_rope_head_stride", C.c_int64),
+                ("n_heads", C.c_int), ("scale", C.c_float), ("tree", C.c_void_p), ("tree_words", C.c_int),
+                ("out", C.c_void_p), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("lse", C.c_void_p)]
+
+
 _vp = C.c_void_p
 _fp = C.POINTER(C.c_float)
 _ip = C.POINTER(C.c_int)
@@ -57,6 +80,15 @@ SIGNATURES = {
     "moe_sample": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_float, C.c_float, C.POINTER(C.c_uint32), _vp]),
     "moe_sample_device": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_float, C.c_float, C.c_uint32, _vp, _vp]),
     "moe_rng_advance": (C.c_uint32, [C.c_uint32, C.c_int]),
+    "moe_kv_row_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "moe_rope_device": (C.c_int, [_vp, C.POINTER(RopeConfigC), _vp, C.c_int, C.c_int64, C.c_int64, _vp, C.c_int,
+                                  C.c_int64, C.c_int64, _vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp]),
+    "moe_kv_write_device": (C.c_int, [_vp, C.POINTER(KVCacheC), C.POINTER(KVBatchC), _vp, C.c_int, C.c_int64, _vp,
+                                      C.c_float, C.POINTER(RopeConfigC), _vp, _vp]),
+    "moe_kv_read_device": (C.c_int, [_vp, C.POINTER(KVCacheC), C.POINTER(KVBatchC), _vp, C.c_int, C.c_int64, _vp]),
+    "moe_mla_workspace_bytes": (C.c_size_t, [_vp, C.c_int]),
+    "moe_mla_attention_device": (C.c_int, [_vp, C.POINTER(KVCacheC), C.POINTER(KVBatchC), C.POINTER(MlaQueryC), _vp,
+                                           C.c_size_t, _vp]),
     "moe_forward": (C.c_int, [_vp, C.c_int, _vp, C.c_int, _vp, _vp, _vp]),
     "moe_forward_device": (C.c_int, [_vp, C.c_int, _vp, C.c_int, _vp, _vp, _vp, _vp]),
     "moe_check_error": (C.c_int, [_vp]),

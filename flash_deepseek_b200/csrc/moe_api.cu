@@ -21,6 +21,7 @@
 #include "../../include/moe_cuda.h"
 #include "moe_common.cuh"
 #include "moe_internal.h"
+#include "moe_kv_host.h"
 #include "moe_nccl.h"
 #include "moe_wait.h"
 
@@ -120,6 +121,7 @@ struct moe_ctx {
     size_t mb_x = 0, mb_meta = 0, mb_y = 0;
     int *ep_done = nullptr;  // [3] block counters of the pack, pre-combine and final kernels
     unsigned long long *d_seq = nullptr;  // peer-exchange steps completed by this rank (device)
+    int sms = 0;             // multiprocessors of the device
     int *hits = nullptr;     // moe_record_expert_hits target, or nullptr
     bool comm_aborted = false;  // a host wait gave up on an NCCL exchange
     bool ep_failed = false;     // a peer-exchange wait gave up: the ranks are out of step
@@ -436,6 +438,7 @@ moe_ctx *moe_create(const moe_config *cfg, int device, int rank, int world_size,
         delete c;
         return nullptr;
     }
+    if (cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) c->sms = 148;
     c->n_local = k.n_experts / world_size;
     c->e0 = rank * c->n_local;
     c->max_tok = k.max_tokens;
@@ -1393,6 +1396,8 @@ static int take_device_error(moe_ctx *c) {
         if (e == EX_ERR_TIMEOUT) return fail(c, MOE_ERR_TIMEOUT, "expert pipeline wait timed out");
         if (e == PF_ERR_TIMEOUT) return fail(c, MOE_ERR_TIMEOUT, "prefill pipeline wait timed out");
         if (e == PF_ERR_PAIR) return fail(c, MOE_ERR_CUDA, "prefill CTA pair: tensor-memory allocations differ");
+        if (e == KV_ERR_TIMEOUT) return fail(c, MOE_ERR_TIMEOUT, "MLA attention pipeline wait timed out");
+        if (e == KV_ERR_BATCH) return fail(c, MOE_ERR_ARG, "cache: page table, page or sequence bounds out of range");
         if (e == MOE_DEV_ERR_INDEX) return fail(c, MOE_ERR_ARG, "expert index out of range in routing");
         return fail(c, MOE_ERR_CUDA, "device error code 0x%x", e);
     }
@@ -1579,6 +1584,93 @@ int moe_sample_device(moe_ctx *c, const float *d_logits, int T, int vocab, float
     if (rc) return rc;
     moe_launch_sample(d_logits, T, vocab, temp, top_p, rng_state, c->sample_p, c->sample_ws, d_tokens,
                       stream ? (cudaStream_t)stream : c->stream, &c->launches);
+    CK(cudaGetLastError());
+    return MOE_OK;
+}
+
+// ---- MLA attention over a paged latent cache (checks: moe_kv_host.h) ---------
+size_t moe_kv_row_bytes(int format, int latent) { return kv_host_row_bytes(format, latent); }
+
+static MoeRopeDev rope_dev(const moe_rope_config *r) {
+    MoeRopeDev d{};
+    d.pairs = r->dim / 2;
+    d.half_layout = r->half_layout ? 1 : 0;
+    d.mscale = r->mscale;
+    kv_rope_turns(r, d.turns);
+    return d;
+}
+static MoeKvDev kv_dev(const moe_kv_cache *kv) {
+    MoeKvDev d{(uint8_t *)kv->data, kv->format, kv->latent, 0, kv->n_pages, (int)kv_host_row_bytes(kv->format, kv->latent)};
+    while ((1 << d.page_shift) < kv->page_size) d.page_shift++;
+    return d;
+}
+static MoeKvBatchDev batch_dev(const moe_kv_batch *b) {
+    return MoeKvBatchDev{b->n_seqs, b->n_tokens, b->q_start, b->ctx_len, b->pages, b->pages_per_seq};
+}
+
+int moe_rope_device(moe_ctx *c, const moe_rope_config *rope, const void *x, int x_type, int64_t xt, int64_t xh,
+                    void *y, int y_type, int64_t yt, int64_t yh, const int *d_pos, int T, int n_heads, int head_dim,
+                    int offset, void *stream) {
+    if (!c) return MOE_ERR_ARG;
+    if (const char *bad = kv_bad_rope_call(rope, x, x_type, xt, xh, y, y_type, yt, yh, d_pos, T, n_heads, head_dim, offset))
+        return fail(c, MOE_ERR_ARG, "moe_rope_device: %s", bad);
+    if (T == 0 || n_heads == 0) return MOE_OK;
+    DeviceScope ds(c->device);
+    moe_launch_rope(rope_dev(rope), x, x_type, xt, xh, y, y_type, yt, yh, d_pos, T, n_heads, head_dim, offset,
+                    stream ? (cudaStream_t)stream : c->stream, &c->launches);
+    CK(cudaGetLastError());
+    return MOE_OK;
+}
+
+int moe_kv_write_device(moe_ctx *c, const moe_kv_cache *kv, const moe_kv_batch *b, const void *x, int type,
+                        int64_t stride, const float *d_norm_w, float eps, const moe_rope_config *rope,
+                        const int *d_pos, void *stream) {
+    if (!c) return MOE_ERR_ARG;
+    const char *bad = kv_bad_cache(kv, b);
+    if (!bad) bad = kv_bad_write(b, x, type, stride, d_norm_w, eps, rope, d_pos);
+    if (bad) return fail(c, MOE_ERR_ARG, "moe_kv_write_device: %s", bad);
+    if (b->n_tokens == 0 || b->n_seqs == 0) return MOE_OK;
+    MoeRopeDev d{};
+    if (rope) d = rope_dev(rope);
+    DeviceScope ds(c->device);
+    moe_launch_kv_write(kv_dev(kv), batch_dev(b), x, type, stride, d_norm_w, eps, rope ? &d : nullptr, d_pos,
+                        c->plan.error, stream ? (cudaStream_t)stream : c->stream, &c->launches);
+    CK(cudaGetLastError());
+    return MOE_OK;
+}
+
+int moe_kv_read_device(moe_ctx *c, const moe_kv_cache *kv, const moe_kv_batch *b, void *y, int type, int64_t stride,
+                       void *stream) {
+    if (!c) return MOE_ERR_ARG;
+    const char *bad = kv_bad_cache(kv, b);
+    if (!bad) bad = kv_bad_read(kv, b, y, type, stride);
+    if (bad) return fail(c, MOE_ERR_ARG, "moe_kv_read_device: %s", bad);
+    if (b->n_tokens == 0 || b->n_seqs == 0) return MOE_OK;
+    DeviceScope ds(c->device);
+    moe_launch_kv_read(kv_dev(kv), batch_dev(b), y, type, stride, c->plan.error,
+                       stream ? (cudaStream_t)stream : c->stream, &c->launches);
+    CK(cudaGetLastError());
+    return MOE_OK;
+}
+
+size_t moe_mla_workspace_bytes(const moe_ctx *c, int latent) {
+    return c && kv_host_row_bytes(MOE_KV_F16, latent) ? moe_mla_ws_bytes(latent, c->sms) : 0;
+}
+
+int moe_mla_attention_device(moe_ctx *c, const moe_kv_cache *kv, const moe_kv_batch *b, const moe_mla_query *q,
+                             void *ws, size_t ws_bytes, void *stream) {
+    if (!c) return MOE_ERR_ARG;
+    const char *bad = kv_bad_cache(kv, b);
+    if (!bad) bad = kv_bad_query(kv, b, q, ws, ws_bytes, moe_mla_ws_bytes(kv->latent, c->sms));
+    if (bad) return fail(c, MOE_ERR_ARG, "moe_mla_attention_device: %s", bad);
+    if (b->n_tokens == 0 || b->n_seqs == 0) return MOE_OK;
+    const MoeMlaQuery dq{q->q_latent, q->q_rope, q->q_latent_token_stride, q->q_latent_head_stride,
+                         q->q_rope_token_stride, q->q_rope_head_stride, q->out, q->out_token_stride,
+                         q->out_head_stride, q->lse, q->tree, q->tree ? q->tree_words : 0, q->n_heads, q->scale};
+    DeviceScope ds(c->device);
+    if (moe_launch_mla(kv_dev(kv), batch_dev(b), dq, ws, c->sms, c->plan.error,
+                       stream ? (cudaStream_t)stream : c->stream, &c->launches))
+        return fail(c, MOE_ERR_CUDA, "moe_mla_attention_device: launch setup failed");
     CK(cudaGetLastError());
     return MOE_OK;
 }

@@ -83,6 +83,8 @@ static inline cudaError_t moe_launch_pdl(void (*kernel)(KArgs...), dim3 grid, di
 #define PF_ERR_TIMEOUT 0x7200        // prefill GEMM pipeline: an mbarrier wait gave up
 #define PF_ERR_PAIR 0x7201           // prefill GEMM: the CTA pair's tensor-memory columns differ
 #define EP_ERR_TIMEOUT 0x7300        // peer exchange: a peer's step flag did not arrive
+#define KV_ERR_BATCH 0x7400          // cache: page table, page or sequence bounds out of range
+#define KV_ERR_TIMEOUT 0x7401        // MLA attention pipeline: an mbarrier wait gave up
 
 // Raises a kernel's dynamic shared-memory limit on the current device when
 // `bytes` exceeds what was set there before.  The attribute belongs to the
@@ -298,6 +300,46 @@ void moe_launch_to_f16(int type, const void *src, __half *dst, size_t n, float *
                        uint64_t *launches);
 void moe_launch_prep_rows(const float *recv, const int *meta, int meta_w, int R, const float *local, int T, int H,
                           uint8_t *xop, cudaStream_t s, uint64_t *launches);
+// ---- MLA attention over a paged latent cache (moe_kv.cu, moe_mla.cu) --------
+// moe_kv_cache / moe_kv_batch of the C ABI as the kernels take them
+struct MoeKvDev {
+    uint8_t *data;
+    int format, latent, page_shift, n_pages, row_bytes;
+};
+struct MoeKvBatchDev {
+    int n_seqs, n_tokens;
+    const int *q_start, *ctx_len, *pages;
+    int pages_per_seq;
+};
+// rotary frequencies of the pairs, in turns (2 pi radians) per position
+struct MoeRopeDev {
+    double turns[128];
+    int pairs, half_layout;
+    float mscale;
+};
+struct MoeMlaQuery {
+    const void *latent, *rope;   // [token][head][latent], [token][head][64]
+    long long lt, lh, rt, rh;    // strides in elements: token, head
+    void *out;                   // [token][head][latent]
+    long long ot, oh;
+    float *lse;                  // [token][head] or nullptr
+    const uint32_t *tree;        // [token][tree_words] or nullptr (causal)
+    int tree_words, n_heads;
+    float scale;
+};
+void moe_launch_rope(const MoeRopeDev &rope, const void *x, int x_type, long long xt, long long xh, void *y,
+                     int y_type, long long yt, long long yh, const int *pos, int n_tokens, int n_heads, int head_dim,
+                     int offset, cudaStream_t s, uint64_t *launches);
+// rope: nullptr keeps the rotary values as given
+void moe_launch_kv_write(const MoeKvDev &kv, const MoeKvBatchDev &b, const void *x, int type, long long stride,
+                         const float *norm_w, float eps, const MoeRopeDev *rope, const int *pos, int *error,
+                         cudaStream_t s, uint64_t *launches);
+void moe_launch_kv_read(const MoeKvDev &kv, const MoeKvBatchDev &b, void *y, int type, long long stride, int *error,
+                        cudaStream_t s, uint64_t *launches);
+size_t moe_mla_ws_bytes(int latent, int sms);
+// 0 = launched; otherwise a driver error while the tensor map was made
+int moe_launch_mla(const MoeKvDev &kv, const MoeKvBatchDev &b, const MoeMlaQuery &q, void *ws, int sms, int *error,
+                   cudaStream_t s, uint64_t *launches);
 // expert parallel (moe_ep.cu)
 void moe_launch_ep_pack(const float *x, const int *idx, const float *w, int T, int K, int H, int world, int n_local,
                         int cap, float *send_x, int *send_meta, int *tok_slot, cudaStream_t s, uint64_t *launches);

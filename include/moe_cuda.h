@@ -235,6 +235,135 @@ int moe_sample_device(moe_ctx *ctx, const float *d_logits, int n_tokens, int voc
 /* The xorshift32 state after n draws (rand_unit, infer.m:412-418). */
 uint32_t moe_rng_advance(uint32_t state, int n);
 
+/* ------------------------------------------- MLA attention, latent cache */
+/* Absorbed multi-head latent attention (mla_forward, infer.m:665-903) over a
+ * paged cache in device memory: the query heads of a token score every row of
+ * latent + 64 values that the token sees, and the output is the weighted mean
+ * of the rows' latent parts, so one cached row serves all heads.  All entry
+ * points take device pointers and are asynchronous on `stream` (NULL = the
+ * context's stream); none allocates, waits or keeps state between calls, so
+ * they can be captured into CUDA graphs, and calls on different streams may
+ * overlap as long as they do not write the same buffers (moe_mla_attention:
+ * the same workspace).  Arguments that live on the device (sequence bounds,
+ * page tables) are checked by the kernels: a token whose row lies outside its
+ * page table, or whose page is out of range, is skipped (moe_kv_write), reads
+ * as zeros (moe_kv_read) or is treated as a row that nobody sees
+ * (moe_mla_attention), and moe_check_error() reports MOE_ERR_ARG. */
+#define MOE_KV_ROPE 64      /* rotary values of a cache row (QK_ROPE_HEAD_DIM) */
+#define MOE_KV_F16 1        /* rows of (latent + 64) fp16 */
+#define MOE_KV_BF16 30      /* rows of (latent + 64) bf16 */
+/* 8-bit rows: `latent` e4m3 codes, 64 rotary values of fp16 / bf16, latent/32
+ * scale bytes (127 + k: the 32 codes of a group stand for code * 2^k, k the
+ * least with amax <= 448 * 2^k, kept in [-15, 7]; larger values saturate, and
+ * a group with an infinity or a NaN reads as NaN), padded to 16 bytes. */
+#define MOE_KV_FP8_F16 101
+#define MOE_KV_FP8_BF16 130
+
+typedef struct moe_kv_cache {
+    void *data;      /* device, 128-byte aligned: [n_pages][page_size] rows of moe_kv_row_bytes() */
+    int format;      /* MOE_KV_* */
+    int latent;      /* KV_LORA_RANK 512; 128, 256, 384 or 512 */
+    int page_size;   /* rows of a page, a power of two in 8 .. 1024 */
+    int n_pages;     /* n_pages * page_size < 2^31 */
+} moe_kv_cache;
+
+/* The rows of a call, packed sequence after sequence: sequence b owns rows
+ * q_start[b] .. q_start[b + 1] - 1 of the call, which are rows ctx_len[b],
+ * ctx_len[b] + 1, ... of the sequence in the cache; row r of sequence b is row
+ * r % page_size of page pages[b][r / page_size].  Sequences may be empty; rows
+ * of the call in front of q_start[0] or from q_start[n_seqs] on belong to no
+ * sequence and are left as they are. */
+typedef struct moe_kv_batch {
+    int n_seqs;          /* 0 .. 4096 */
+    int n_tokens;        /* rows of the call's buffers */
+    const int *q_start;  /* device [n_seqs + 1], ascending */
+    const int *ctx_len;  /* device [n_seqs] */
+    const int *pages;    /* device [n_seqs][pages_per_seq] */
+    int pages_per_seq;
+} moe_kv_batch;
+
+/* Rotary frequencies (yarn_init_once / yarn_freq, infer.m:590-624): pair i of
+ * dim / 2 turns by theta^(-2 i / dim) radians per position; with scale > 1
+ * (YaRN) the frequencies whose wavelength exceeds orig_ctx / beta_slow are
+ * divided by scale, those below orig_ctx / beta_fast kept, a linear ramp over
+ * the pair index between.  cos and sin are multiplied by mscale. */
+typedef struct moe_rope_config {
+    int dim;          /* rotated values, even, 2 .. 256 */
+    int half_layout;  /* 0: pairs (2i, 2i + 1); 1: pairs (i, i + dim / 2) */
+    float theta;      /* 10000 */
+    float scale;      /* 1 = no scaling; 40 (ROPE_SCALE) */
+    float orig_ctx;   /* 4096 */
+    float beta_fast, beta_slow;  /* 32, 1 */
+    float mscale;     /* 1 */
+} moe_rope_config;
+
+/* Bytes of one cache row; 0 for a format or size that is not supported. */
+size_t moe_kv_row_bytes(int format, int latent);
+
+/* Rotary positions: y = x with values [offset, offset + dim) of every head
+ * rotated by its token's position, the others copied.  x, y: [n_tokens]
+ * [n_heads][head_dim] of MOE_TYPE_F32 / F16 / BF16 with the given strides in
+ * elements (token, head), the values of a head contiguous.  y may be x (same
+ * type and strides: only the rotated values are touched); otherwise the two
+ * must not overlap.  d_pos: device int [n_tokens], any value.  The angle is
+ * formed in 64 bits, so far positions lose nothing. */
+int moe_rope_device(moe_ctx *ctx, const moe_rope_config *rope, const void *d_x, int x_type,
+                    int64_t x_token_stride, int64_t x_head_stride, void *d_y, int y_type,
+                    int64_t y_token_stride, int64_t y_head_stride, const int *d_pos, int n_tokens,
+                    int n_heads, int head_dim, int offset, void *stream);
+
+/* Appends rows to the cache: per row of `latent` + 64 values (kv_a of the
+ * token, MOE_TYPE_F32 / F16 / BF16, rows row_stride elements apart) the latent
+ * part through RMSNorm (weight fp32 [latent], NULL: as given), the rest
+ * rotated to position d_pos[row] (rope NULL: as given; rope->dim must be 64),
+ * both stored in the cache's format.  Which row goes where: moe_kv_batch.  Two
+ * rows of one call that map to the same cache row (a page listed twice) leave
+ * that row undefined. */
+int moe_kv_write_device(moe_ctx *ctx, const moe_kv_cache *kv, const moe_kv_batch *batch, const void *d_kv_a,
+                        int type, int64_t row_stride, const float *d_norm_w, float eps,
+                        const moe_rope_config *rope, const int *d_pos, void *stream);
+
+/* Reads rows back as values: row i of sequence b of the batch, of latent + 64
+ * values, to d_out + (q_start[b] + i) * row_stride. */
+int moe_kv_read_device(moe_ctx *ctx, const moe_kv_cache *kv, const moe_kv_batch *batch, void *d_out, int type,
+                       int64_t row_stride, void *stream);
+
+/* Absorbed attention of the batch's tokens over the cache, for all heads:
+ *   s[r] = scale * (q_latent . latent[r] + q_rope . rope[r]),
+ *   out = sum_r softmax(s)[r] * latent[r],  lse = log sum_r exp(s[r])
+ * over the rows r that the token sees: every row below ctx_len of its
+ * sequence, and of the call's own rows (which moe_kv_write put at ctx_len,
+ * ctx_len + 1, ...) those that its tree bits name: bit j % 32 of
+ * d_tree[token][j / 32] for the j-th row of its sequence in this call, itself
+ * included.  d_tree NULL: a causal chain (j <= its own number).  Rows that a
+ * token does not see never touch its output, whatever they hold; a visible
+ * row with an infinity or a NaN makes it NaN.  A token that sees nothing gets
+ * out = 0 and lse = -infinity.
+ * q_latent [token][head][latent], q_rope [token][head][64], out
+ * [token][head][latent] in the cache's 16-bit type (fp16 for MOE_KV_F16 and
+ * MOE_KV_FP8_F16, else bf16), strides in elements (multiples of 8), buffers
+ * 16-byte aligned; d_lse fp32 [n_tokens][n_heads] or NULL.  Products of 16-bit
+ * operands, sums and softmax statistics in fp32; probabilities are rounded to
+ * the 16-bit type before they weight the rows.
+ * Workspace: moe_mla_workspace_bytes(ctx, latent), 256-byte aligned, needs no
+ * initialisation, one for each call that may run at the same time. */
+typedef struct moe_mla_query {
+    const void *q_latent;
+    int64_t q_latent_token_stride, q_latent_head_stride;
+    const void *q_rope;
+    int64_t q_rope_token_stride, q_rope_head_stride;
+    int n_heads;           /* 1 .. 1024 */
+    float scale;
+    const uint32_t *tree;  /* device [n_tokens][tree_words] or NULL */
+    int tree_words;        /* at least the longest sequence's rows / 32 */
+    void *out;
+    int64_t out_token_stride, out_head_stride;
+    float *lse;
+} moe_mla_query;
+size_t moe_mla_workspace_bytes(const moe_ctx *ctx, int latent);
+int moe_mla_attention_device(moe_ctx *ctx, const moe_kv_cache *kv, const moe_kv_batch *batch,
+                             const moe_mla_query *q, void *d_workspace, size_t workspace_bytes, void *stream);
+
 /* ---------------------------------------------------------------- forward */
 /* The full MoE block for n_tokens tokens held by this rank (host buffers):
  * out[t] = sum_k w_k E_{idx_k}(h[t]) + shared(h[t]), fp32 [n_tokens x H].
