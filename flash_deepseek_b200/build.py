@@ -15,7 +15,7 @@ ROOT = os.path.dirname(HERE)
 OUT = os.path.join(HERE, "libmoe_cuda.so")
 SOURCES = ["moe_kernels.cu", "moe_experts.cu", "moe_experts_tc.cu", "moe_prefill.cu", "moe_ep.cu", "moe_api.cu",
            "moe_noalloc.cu", "moe_dense.cu", "moe_sample.cu", "moe_kv.cu", "moe_mla.cu"]
-HEADERS = ["moe_common.cuh", "moe_internal.h", "moe_kv.cuh", "moe_kv_host.h", "moe_nccl.h", "moe_umma.cuh", "moe_wait.h"]
+HEADERS = ["moe_common.cuh", "moe_internal.h", "moe_kv.cuh", "moe_kv_host.h", "moe_kv_plan.h", "moe_nccl.h", "moe_umma.cuh", "moe_wait.h"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",

@@ -75,3 +75,13 @@ def test_quantize_reference():
 
 def E(codes):
     return R.E4M3[codes]
+
+
+def test_work_division(tmp_path):
+    exe = str(tmp_path / "kv_plan")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-Wno-unknown-pragmas", os.path.join(ROOT, "tests", "kv_plan.cc"),
+                    "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.startswith("ok"), r.stdout
+    cut, whole = int(r.stdout.split()[1]), int(r.stdout.split()[3])
+    assert cut > 1000 and whole > 1000
