@@ -41,21 +41,29 @@ namespace {
 
 constexpr int MLA_CHUNK = MLA_N * 128;      // bytes of a 64-row x 64-value chunk
 constexpr int MLA_QCHUNK = MLA_M * 128;     // bytes of a 128-row x 64-value query chunk
-constexpr int MLA_RA = 8;                   // chunks of ring A
+constexpr int MLA_RA = 6;                   // chunks of ring A
 constexpr int MLA_SB = 3;                   // tiles of ring B
-constexpr int MLA_TM_S = 256, MLA_TM_P = 320, MLA_TM_Q = 352;   // tensor-memory columns (the output from 0)
+// Tensor-memory columns: the output from 0 (at most 256), two score tiles of 64 (the weights of a tile, 32 columns of
+// 16-bit pairs, take the place of its scores), the query's chunks.
+constexpr int MLA_TM_S = 256, MLA_TM_Q = 384;
 constexpr float MLA_RAISE = 8.0f;           // log2: how far scores may pass the reference before it is raised
 
 // Tensor memory left for query chunks of 32 columns (64 values) each: all of
-// them for up to 384 latent values, 5 of 9 for 512.
+// them for up to 256 latent values, 6 of 7 for 384, 4 of 9 for 512.
 __host__ __device__ constexpr int mla_q_tm(int latent) {
     const int all = latent / 64 + 1, fit = (512 - MLA_TM_Q + (256 - latent / 2)) / 32;
     return all < fit ? all : fit;
 }
 
+// Query chunks in shared memory: the others, one at least (the way of all into tensor memory)
+__host__ __device__ constexpr int mla_q_sm(int latent) {
+    const int rest = latent / 64 + 1 - mla_q_tm(latent);
+    return rest > 1 ? rest : 1;
+}
+
 struct MlaCtl {   // control block behind the tiles
-    uint64_t full_a[MLA_RA], empty_a[MLA_RA], full_b[MLA_SB], empty_b[MLA_SB];
-    uint64_t s_full, s_empty, p_full, pv_done, q_ready, drain;
+    uint64_t full_a[MLA_RA], empty_a[MLA_RA], full_b[MLA_SB], empty_b[MLA_SB];   // chunks of ring A, tiles of ring B
+    uint64_t s_full[2], p_full[2], pv_done[2], q_ready, drain;   // by tile parity
     uint64_t nonfinite[2];       // by tile parity: rows of a tile with an infinity or a NaN in this CTA's latent half
     uint8_t valid[MLA_SB][8];    // 8-row groups of a tile whose page exists
     int64_t w0, w1, off0;        // the pair's share: first and last tile, place of the first in its sequence
@@ -110,6 +118,24 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// two fp32 values in one 64-bit register, one instruction for both
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t r, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // 4 e4m3 codes times a group's scale as 4 16-bit values.  The code's exponent
 // and mantissa bits placed in the 16-bit format's fields are the value over
 // 2^120 (bf16) or 2^8 (fp16), subnormals too; f holds 2^(120 + k) or 2^(8 + k).
@@ -161,9 +187,9 @@ __device__ __forceinline__ uint64_t mla_visible(const MoeMlaQuery &q, const MlaS
 }
 
 // ---------------------------------------------------------------------------
-template <bool BF16, bool FP8>
+template <bool BF16, bool FP8, int NV>   // NV: latent chunks (of 64 values) of a CTA's half
 struct MlaKernel {
-    static constexpr int THREADS = FP8 ? 512 : 256;
+    static constexpr int NC = 2 * NV + 1, NQ = mla_q_tm(128 * NV);   // chunks of a row; of the query in tensor memory
 
     const MoeKvDev &kv;
     const MlaSeqAt &seq_at;
@@ -173,12 +199,12 @@ struct MlaKernel {
     int *error;
     uint8_t *ring_b, *ring_a, *sq;
     MlaCtl *c;
-    int half, pair, pairs, nv, nc, nq;   // latent chunks of a half, chunks of a row, query chunks in tensor memory
+    int half, pair;
     int lane, warp;
 
     // the chunk (64 values of a row) at place p of the order: own half, other half, rotary
     __device__ __forceinline__ int chunk_at(int p) const {
-        return p < nv ? half * nv + p : p < 2 * nv ? (1 - half) * nv + p - nv : 2 * nv;
+        return p < NV ? half * NV + p : p < 2 * NV ? (1 - half) * NV + p - NV : 2 * NV;
     }
     __device__ __forceinline__ MlaWalk walk() const {
         MlaWalk w{};
@@ -226,12 +252,12 @@ struct MlaKernel {
                 if (!tc_wait_warp(&c->empty_b[st], (ib / MLA_SB + 1) & 1)) return stop_tma(ia, ib);
                 if (lane < 8) c->valid[st][lane] = ok;
                 __syncwarp();
-                if (lane == 0) tc_expect(&c->full_b[st], (uint32_t)nv * MLA_CHUNK);
+                if (lane == 0) tc_expect(&c->full_b[st], (uint32_t)NV * MLA_CHUNK);
                 __syncwarp();
                 if (box)
-                    for (int p = 0; p < nv; p++)
-                        tc_tma2(ring_b + (st * nv + p) * MLA_CHUNK + off, tm, chunk_at(p) * 64, row, &c->full_b[st]);
-                for (int p = nv; p < nc; p++, ia++) {
+                    for (int p = 0; p < NV; p++)
+                        tc_tma2(ring_b + (st * NV + p) * MLA_CHUNK + off, tm, chunk_at(p) * 64, row, &c->full_b[st]);
+                for (int p = NV; p < NC; p++, ia++) {
                     const int sa = ia % MLA_RA;
                     if (!tc_wait_warp(&c->empty_a[sa], (ia / MLA_RA + 1) & 1)) return stop_tma(ia, ib + 1);
                     if (lane == 0) tc_expect(&c->full_a[sa], MLA_CHUNK);
@@ -245,11 +271,12 @@ struct MlaKernel {
     // ---- loads, 8-bit formats: 8 warps, 4 threads per row, 16 codes of every chunk each.  The next tile's
     // loads are issued as this tile's chunks are expanded, so a tile's bytes are always in flight.
     __device__ void produce_expand() {
-        const int tid = threadIdx.x - 256, r = tid >> 2, qd = tid & 3, L = kv.latent;
+        constexpr int L = 128 * NV;
+        const int tid = threadIdx.x - 256, r = tid >> 2, qd = tid & 3;
         MlaWalk w = walk();
         MlaSeg g;
         int ia = 0, ib = 0;
-        uint4 code[8], rope[2], sc;
+        uint4 code[2 * NV], rope[2], sc;
         const uint4 zero = make_uint4(0, 0, 0, 0);
         // loads of tile t of the current segment
         const uint8_t *row;
@@ -276,8 +303,7 @@ struct MlaKernel {
         locate(g.seq, w.s, t);
         load_sc();
 #pragma unroll
-        for (int p = 0; p < 8; p++)
-            if (p < 2 * nv) code[p] = load_code(p);
+        for (int p = 0; p < 2 * NV; p++) code[p] = load_code(p);
         rope[0] = load_rope(0), rope[1] = load_rope(1);
         for (bool more = true; more; ib++) {
             const int st = ib % MLA_SB;
@@ -299,18 +325,17 @@ struct MlaKernel {
             const uint32_t sw = (uint32_t)(r & 7);
             const uint32_t at = (uint32_t)(r >> 3) * 1024 + sw * 128;
 #pragma unroll
-            for (int p = 0; p < 9; p++) {
-                if (p >= nc) break;
+            for (int p = 0; p < NC; p++) {
                 uint8_t *dst;
-                if (p < nv) dst = ring_b + (st * nv + p) * MLA_CHUNK;
+                if (p < NV) dst = ring_b + (st * NV + p) * MLA_CHUNK;
                 else {
                     const int sa = ia % MLA_RA;
                     if (!tc_wait_warp(&c->empty_a[sa], (ia / MLA_RA + 1) & 1)) return give_up();
                     dst = ring_a + sa * MLA_CHUNK;
                 }
                 uint4 lo, hi;
-                if (p < 2 * nv) {
-                    const uint4 v = code[p < 8 ? p : 7];
+                if (p < 2 * NV) {
+                    const uint4 v = code[p < 2 * NV ? p : 0];
                     const int grp = 2 * chunk_at(p) + (qd >> 1);
                     const uint32_t word = grp < 4 ? s4.x : grp < 8 ? s4.y : grp < 12 ? s4.z : s4.w;
                     const uint32_t f = scale2<BF16>(word >> (8 * (grp & 3)) & 255);
@@ -318,7 +343,7 @@ struct MlaKernel {
                     const uint2 d = expand4<BF16>(v.z, f), e = expand4<BF16>(v.w, f);
                     lo = make_uint4(a.x, a.y, b.x, b.y);
                     hi = make_uint4(d.x, d.y, e.x, e.y);
-                    if (p < 8) code[p] = load_code(p);
+                    code[p < 2 * NV ? p : 0] = load_code(p);
                 } else {
                     lo = rope[0], hi = rope[1];
                     rope[0] = load_rope(0), rope[1] = load_rope(1);
@@ -328,143 +353,169 @@ struct MlaKernel {
                 *reinterpret_cast<uint4 *>(dst + at + ((2 * qd + 1) ^ sw) * 16) = hi;
                 fence_async_smem();
                 __syncwarp();
-                if (p >= nv) {
+                if (p >= NV) {
                     if (lane == 0) tc_arrive(&c->full_a[ia % MLA_RA]);
                     ia++;
-                } else if (p == nv - 1) {
+                } else if (p == NV - 1) {
                     if (lane == 0) tc_arrive(&c->full_b[st]);
                 }
             }
         }
     }
 
-    // ---- MMA issue: one warp, every lane runs the loop, an elected lane issues
+    // ---- MMA issue: one warp, every lane runs the loop, an elected lane issues.  Operands are broadcast from lane 0
+    // and every branch goes by a vote: where the compiler cannot prove operands and control flow uniform, an MMA takes
+    // 90 cycles to issue, against 32 (scores) to run.
+    // Barriers are tested ahead, before the MMAs in front of their use: a test of a completed phase takes 100 cycles
+    // from issue to branch, which the tensor pipe would stand idle.
+    __device__ __forceinline__ bool then_wait(uint32_t seen, uint64_t *b, uint32_t parity) {
+        return __all_sync(0xffffffffu, seen) || tc_wait_warp(b, parity);
+    }
+    struct Issue {
+        uint32_t tmem, rb, ra, sq;         // base addresses
+        int st, sa, phase_b, phase_a;      // next tile's stage and next chunk's slot, their parities
+        uint32_t seen_b;                   // the test of the next tile's ring B stage
+    };
+    // the weights of tile i times its latent chunks; nb: the stage's parity of the tile behind
+    __device__ bool output(Issue &x, int i, int st, uint32_t seen, uint32_t more) {
+        constexpr uint32_t id = umma_idesc_16(MLA_M, 64 * NV, BF16, 1);
+        if (!then_wait(seen, &c->p_full[i & 1], (i >> 1) & 1)) return false;
+        x.seen_b = tc_test(&c->full_b[x.st], x.phase_b);
+        tmem_fence_after();
+        const uint32_t ts = x.tmem + MLA_TM_S + (i & 1) * 64;
+        const uint64_t d = umma_desc_sw128_mn(x.rb + st * NV * MLA_CHUNK, MLA_CHUNK);
+#pragma unroll
+        for (int k = 0; k < MLA_N / 16; k++)   // 16 cache rows: 2048 bytes of the tile, 8 columns of weights
+            umma_f16_ta_warp(x.tmem, ts + k * 8, d + k * (2048 >> 4), id, k == 0 ? more : 1u);
+        umma_commit_warp(&c->empty_b[st]);
+        umma_commit_warp(&c->pv_done[i & 1]);
+        return true;
+    }
+    // the scores of tile `it`; `seen`: the test of the weights of the tile before, made before the last chunk
+    __device__ bool scores(Issue &x, int it, uint32_t &seen) {
+        constexpr uint32_t id = umma_idesc_16(MLA_M, MLA_N, BF16, 0);
+        if (!then_wait(x.seen_b, &c->full_b[x.st], x.phase_b)) return false;
+        uint32_t seen_a = 0;
+        tmem_fence_after();
+        const uint64_t a0 = umma_desc_sw128(x.sq);
+        // The score tile it & 1 is free: its weights' product (tile it - 2) was issued before, and the tensor pipe
+        // runs in order
+        const uint32_t ts = x.tmem + MLA_TM_S + (it & 1) * 64;
+#pragma unroll
+        for (int p = 0; p < NC; p++) {
+            if (p >= NV && !then_wait(seen_a, &c->full_a[x.sa], x.phase_a)) return false;
+            const int sa = x.sa;
+            const uint64_t b = umma_desc_sw128(p < NV ? x.rb + (x.st * NV + p) * MLA_CHUNK : x.ra + sa * MLA_CHUNK);
+            if (p >= NV && ++x.sa == MLA_RA) x.sa = 0, x.phase_a ^= 1;
+            if (p >= NV - 1 && p < NC - 1) seen_a = tc_test(&c->full_a[x.sa], x.phase_a);
+            if (p == NC - 1) seen = tc_test(&c->p_full[(it - 1) & 1], ((it - 1) >> 1) & 1);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (p < NQ) umma_f16_ta_warp(ts, x.tmem + q_col(p) + k * 8, b + k * 2, id, p > 0 || k > 0);
+                else umma_f16_warp(ts, a0 + (p - NQ) * (MLA_QCHUNK >> 4) + k * 2, b + k * 2, id, p > 0 || k > 0);
+            }
+            if (p >= NV) umma_commit_warp(&c->empty_a[sa]);
+        }
+        umma_commit_warp(&c->s_full[it & 1]);
+        if (++x.st == MLA_SB) x.st = 0, x.phase_b ^= 1;
+        return true;
+    }
     __device__ void issue() {
-        const uint32_t tmem = c->tmem;
-        const uint32_t id_s = umma_idesc_16(MLA_M, MLA_N, BF16, 0), id_o = umma_idesc_16(MLA_M, kv.latent / 2, BF16, 1);
+        Issue x{uni(c->tmem), uni(umma_smem_u32(ring_b)), uni(umma_smem_u32(ring_a)), uni(umma_smem_u32(sq)), 0, 0, 0, 0, 0};
         MlaWalk w = walk();
         MlaSeg g;
-        int ia = 0, it = 0, seg = 0;   // ring A chunks, tiles, segments so far
-        auto output = [&](int i, bool first) -> bool {
-            const int st = i % MLA_SB;
-            if (!tc_wait_warp(&c->p_full, i & 1)) return false;
-            tmem_fence_after();
-            const uint64_t d = umma_desc_sw128_mn(umma_smem_u32(ring_b + st * nv * MLA_CHUNK), MLA_CHUNK);
-#pragma unroll
-            for (int k = 0; k < MLA_N / 16; k++)   // 16 cache rows: 2048 bytes of the tile, 8 columns of P
-                umma_f16_ta_warp(tmem, tmem + MLA_TM_P + k * 8, d + k * (2048 >> 4), id_o, !(first && k == 0));
-            umma_commit_warp(&c->empty_b[st]);
-            umma_commit_warp(&c->pv_done);
-            return true;
-        };
+        int it = 0, seg = 0, prev = 0;   // tiles, segments so far; the stage of the tile before
+        uint32_t seen = 0;
         bool ok = true;
-        while (ok && w.next(g, seq_at)) {
+        while (__all_sync(0xffffffffu, ok && w.next(g, seq_at))) {
+            const int n = uni(g.tile1 - g.tile0);
             ok = tc_wait_warp(&c->q_ready, seg & 1);
             seg++;
-            if (!ok) break;
-            for (int t = g.tile0; ok && t < g.tile1; t++, it++) {
-                const int st = it % MLA_SB;
-                ok = (it == 0 || tc_wait_warp(&c->s_empty, (it - 1) & 1)) && tc_wait_warp(&c->full_b[st], (it / MLA_SB) & 1);
-                if (!ok) break;
-                tmem_fence_after();
-                for (int p = 0; p < nc; p++) {
-                    const uint8_t *src;
-                    if (p < nv) src = ring_b + (st * nv + p) * MLA_CHUNK;
-                    else {
-                        const int sa = ia % MLA_RA;
-                        ok = tc_wait_warp(&c->full_a[sa], (ia / MLA_RA) & 1);
-                        if (!ok) break;
-                        src = ring_a + sa * MLA_CHUNK;
-                    }
-                    const uint64_t b = umma_desc_sw128(umma_smem_u32(src));
-                    if (p < nq) {
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            umma_f16_ta_warp(tmem + MLA_TM_S, tmem + q_col(p) + k * 8, b + k * 2, id_s, p > 0 || k > 0);
-                    } else {
-                        const uint64_t a = umma_desc_sw128(umma_smem_u32(sq + (p - nq) * MLA_QCHUNK));
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            umma_f16_warp(tmem + MLA_TM_S, a + k * 2, b + k * 2, id_s, p > 0 || k > 0);
-                    }
-                    if (p >= nv) umma_commit_warp(&c->empty_a[ia++ % MLA_RA]);
-                }
-                if (!ok) break;
-                umma_commit_warp(&c->s_full);
-                if (t > g.tile0) ok = output(it - 1, t - 1 == g.tile0);
+            for (int t = 0; __all_sync(0xffffffffu, ok && t < n); t++, it++) {
+                const int st = x.st;
+                ok = scores(x, it, seen);
+                if (__all_sync(0xffffffffu, ok && t > 0)) ok = output(x, it - 1, prev, seen, t > 1);
+                prev = st;
             }
-            if (ok) ok = output(it - 1, g.tile1 - 1 == g.tile0);
+            if (__all_sync(0xffffffffu, ok)) ok = output(x, it - 1, prev, 0, n > 1);
         }
         if (!ok) give_up();
         // nothing of this warp's is in flight when the CTA ends
         umma_commit_warp(&c->drain);
         tc_wait_warp(&c->drain, 0);
     }
+    static __device__ __forceinline__ uint32_t uni(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
     // tensor-memory column of the query chunk at place p
-    __device__ __forceinline__ uint32_t q_col(int p) const {
+    static __device__ __forceinline__ uint32_t q_col(int p) {
         // below 512 latent values the output takes fewer columns: the first chunks go behind it
-        const int spare = (256 - kv.latent / 2) / 32;
-        return p < spare ? kv.latent / 2 + p * 32 : MLA_TM_Q + (p - spare) * 32;
+        constexpr int spare = (256 - 64 * NV) / 32;
+        return p < spare ? 64 * NV + p * 32 : MLA_TM_Q + (p - spare) * 32;
     }
+
+    // The output product of tile i is done.  Each parity has a barrier: this warp has seen the scores of tile i or i + 1,
+    // so the product of tile i - 2 is done and the barrier at most one phase behind (a wait by parity that is two phases
+    // behind would never end).
+    __device__ __forceinline__ bool output_done(int i) { return tc_wait_warp(&c->pv_done[i & 1], (i >> 1) & 1); }
 
     // ---- softmax and output: 4 warps, one query row per thread
     __device__ void rows() {
         const uint32_t tmem = c->tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const int r = (warp & 3) * 32 + lane, L = kv.latent, half_cols = L / 2;
-        const float c2 = q.scale * 1.4426950408889634f;
+        const int r = (warp & 3) * 32 + lane, L = 128 * NV, half_cols = 64 * NV;
+        // scores in units of log2: a negative scale flips the query's signs, a scale of zero makes the query zero, so
+        // that the factor is positive and the largest product gives the largest score
+        const float c2 = q.scale == 0.0f ? 1.0f : fabsf(q.scale) * 1.4426950408889634f;
         MlaWalk w = walk();
         MlaSeg g;
         int it = 0;
         bool ok = true;
         while (ok && w.next(g, seq_at)) {
             const MlaSeq s = w.s;
-            const int64_t row = (int64_t)g.block * MLA_M + r;
-            const bool live = row < (int64_t)s.n * q.n_heads;
-            const int token = live ? (int)(row / q.n_heads) : 0, head = live ? (int)(row - (int64_t)token * q.n_heads) : 0;
-            load_query(r, live, (int64_t)s.q0 + token, head);
+            const uint32_t row = (uint32_t)g.block * MLA_M + r;
+            const bool live = row < (uint32_t)s.n * q.n_heads;
+            const int token = live ? row / (uint32_t)q.n_heads : 0, head = live ? row - (uint32_t)token * q.n_heads : 0;
+            load_query(r, s, (uint32_t)g.block * MLA_M);
             float ref = -INFINITY, l = 0.0f;
             for (int t = g.tile0; t < g.tile1; t++, it++) {
                 const int st = it % MLA_SB;
                 const int64_t pos0 = (int64_t)t * MLA_N;
-                ok = tc_wait_warp(&c->s_full, it & 1);
+                ok = tc_wait_warp(&c->s_full[it & 1], (it >> 1) & 1);
                 if (!ok) break;
                 tmem_fence_after();
-                float v[64];
-                tmem_ld32(tmem + MLA_TM_S, *reinterpret_cast<float(*)[32]>(v));
-                tmem_ld32(tmem + MLA_TM_S + 32, *reinterpret_cast<float(*)[32]>(v + 32));
-                tmem_fence_before();
-                __syncwarp();
-                if (lane == 0) tc_arrive(&c->s_empty);
                 // a tile that reaches the drafted rows, or lacks a page: hide what the row does not see
-                ok = tc_wait_warp(&c->full_b[st], (it / MLA_SB) & 1);   // long complete: orders the valid bytes
-                if (!ok) break;
-#pragma unroll
-                for (int k = 0; k < 64; k++) v[k] *= c2;
                 const uint64_t pages = *reinterpret_cast<const volatile uint64_t *>(c->valid[st]);
-                if (pos0 + MLA_N > s.ctx || pages != 0x0101010101010101ull) {
-                    uint64_t see = mla_visible(q, s, token, pos0) & pages * 255;
-                    const uint64_t nf = clean(st, it & 1);
+                uint64_t see = ~0ull, nf = 0;
+                const bool part = pos0 + MLA_N > s.ctx || pages != 0x0101010101010101ull;
+                if (part) {
+                    see = mla_visible(q, s, token, pos0) & pages * 255;
+                    nf = clean(st, it & 1);
+                }
+                // the scores are read twice (largest, weights), half a tile at a time: all 64 and the weights at once
+                // do not fit 128 registers beside the rest
+                const uint32_t ts = tmem + MLA_TM_S + (it & 1) * 64;
+                float v[32], top = -INFINITY;
 #pragma unroll
-                    for (int k = 0; k < 64; k++) {
-                        if (nf >> k & 1) v[k] = __uint_as_float(0x7FC00000u);
-                        if (!(see >> k & 1)) v[k] = -INFINITY;
+                for (int h = 0; h < 2; h++) {
+                    tmem_ld32(ts + 32 * h, v);
+                    if (part) hide(v, (uint32_t)(see >> 32 * h), (uint32_t)(nf >> 32 * h));
+                    float m0 = fmaxf(fmaxf(top, v[0]), v[1]), m1 = fmaxf(fmaxf(v[2], v[3]), v[4]);
+#pragma unroll
+                    for (int k = 5; k < 29; k += 4) {
+                        m0 = fmaxf(fmaxf(m0, v[k]), v[k + 1]);
+                        m1 = fmaxf(fmaxf(m1, v[k + 2]), v[k + 3]);
                     }
+                    m0 = fmaxf(fmaxf(m0, v[29]), v[30]);
+                    top = fmaxf(fmaxf(m0, m1), v[31]);
                 }
-                float mx[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-                for (int k = 4; k < 64; k++) mx[k & 3] = fmaxf(mx[k & 3], v[k]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                if (it > 0) {   // the previous output product is done: P may be written, the output rescaled
-                    ok = tc_wait_warp(&c->pv_done, (it - 1) & 1);
-                    if (!ok) break;
-                    tmem_fence_after();
-                }
+                top *= c2;
                 if (t == g.tile0) ref = top;
                 else if (__any_sync(0xffffffffu, top > ref + MLA_RAISE)) {
                     // raise the reference: weights stay below 2^8 of it, so fp16 and bf16 hold them
                     const float m = fmaxf(ref, top), f = m == -INFINITY ? 1.0f : ex2(ref - m);
                     l *= f;
                     ref = m;
+                    ok = output_done(it - 1);   // the output holds all tiles before this one
+                    if (!ok) break;
+                    tmem_fence_after();
                     for (int col = 0; col < half_cols; col += 32) {
                         float o[32];
                         uint32_t u[32];
@@ -475,25 +526,36 @@ struct MlaKernel {
                     }
                     tmem_wait_st();
                 }
-                const float m0 = ref == -INFINITY ? 0.0f : ref;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const float m0 = ref == -INFINITY ? 0.0f : -ref;
+                const uint64_t cc = pair2(c2, c2), mm = pair2(m0, m0);
+                uint64_t sum[2] = {0, 0};
                 uint32_t pk[32];
 #pragma unroll
-                for (int k = 0; k < 64; k += 2) {
-                    const float a = ex2(v[k] - m0), b = ex2(v[k + 1] - m0);
-                    sum[k & 2] += a;
-                    sum[(k & 2) + 1] += b;
-                    pk[k / 2] = pack2<BF16>(a, b);
+                for (int h = 1; h >= 0; h--) {
+                    if (h == 0) {   // the second half is still in registers from the first pass
+                        tmem_ld32(ts, v);
+                        if (part) hide(v, (uint32_t)see, (uint32_t)nf);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) {
+                        float a, b;
+                        unpair2(fma2(pair2(v[k], v[k + 1]), cc, mm), a, b);
+                        a = ex2(a), b = ex2(b);
+                        sum[k >> 1 & 1] = add2(sum[k >> 1 & 1], pair2(a, b));
+                        pk[16 * h + k / 2] = pack2<BF16>(a, b);
+                    }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_st32(tmem + MLA_TM_P, pk);
+                float sa, sb;
+                unpair2(add2(sum[0], sum[1]), sa, sb);
+                l += sa + sb;
+                tmem_st32(ts, pk);
                 tmem_wait_st();
                 tmem_fence_before();
                 __syncwarp();
-                if (lane == 0) tc_arrive(&c->p_full);
+                if (lane == 0) tc_arrive(&c->p_full[it & 1]);
             }
             if (!ok) break;
-            ok = tc_wait_warp(&c->pv_done, (it - 1) & 1);
+            ok = output_done(it - 1);
             if (!ok) break;
             tmem_fence_after();
             if (g.whole) store_out(tmem, live, (int64_t)s.q0 + token, head, ref, l);
@@ -502,27 +564,64 @@ struct MlaKernel {
         if (!ok) give_up();
     }
 
-    // The query row into tensor memory and shared memory (zeros behind the block's last row)
-    __device__ __forceinline__ void load_query(int r, bool live, int64_t token, int head) {
-        const uint4 *ql = reinterpret_cast<const uint4 *>(reinterpret_cast<const __half *>(q.latent) + token * q.lt + head * q.lh);
-        const uint4 *qr = reinterpret_cast<const uint4 *>(reinterpret_cast<const __half *>(q.rope) + token * q.rt + head * q.rh);
-        const uint32_t tmem = c->tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        for (int p = 0; p < nc; p++) {
+    // Scores of rows that are not seen become -infinity, of seen ones that hold an infinity or a NaN a NaN
+    static __device__ __forceinline__ void hide(float (&v)[32], uint32_t see, uint32_t nf) {
+#pragma unroll
+        for (int k = 0; k < 32; k++) {
+            if (nf >> k & 1) v[k] = __uint_as_float(0x7FC00000u);
+            if (!(see >> k & 1)) v[k] = -INFINITY;
+        }
+    }
+
+    // The block's query rows into tensor memory and shared memory (zeros behind the last row).  A warp loads its own 32
+    // rows, 8 lanes per 128-byte line (a lane per row touches 32 lines with every load: 11,000 cycles a block), so a chunk
+    // for tensor memory passes through shared memory once, from lanes across a row to a lane per row.
+    __device__ __forceinline__ void load_query(int r, const MlaSeq &s, uint32_t row0) {
+        const uint32_t rows = (uint32_t)s.n * q.n_heads;   // below 2^31, as n_tokens * n_heads is
+        const uint32_t flip = q.scale < 0.0f ? 0x80008000u : 0u, tmem = c->tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const __half *ql[8], *qr[8];   // this lane's piece of rows lane / 8 + 4 i
+        bool live[8];
+        const int u = lane & 7;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t row = row0 + (r & ~31) + (lane >> 3) + 4 * i;
+            live[i] = row < rows && q.scale != 0.0f;
+            const uint32_t token = live[i] ? row / (uint32_t)q.n_heads : 0, head = live[i] ? row - token * q.n_heads : 0;
+            ql[i] = reinterpret_cast<const __half *>(q.latent) + (int64_t)(s.q0 + token) * q.lt + head * q.lh + u * 8;
+            qr[i] = reinterpret_cast<const __half *>(q.rope) + (int64_t)(s.q0 + token) * q.rt + head * q.rh + u * 8;
+        }
+        constexpr int D = FP8 ? 2 : 3;   // chunks in flight
+        uint4 xs[D][8];
+        auto load = [&](int p, uint4 (&x)[8]) {
             const int g = chunk_at(p);
-            const uint4 *src = g < 2 * nv ? ql + g * 8 : qr;
-            uint32_t u[32];
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const uint4 x = live ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
-                u[4 * k] = x.x, u[4 * k + 1] = x.y, u[4 * k + 2] = x.z, u[4 * k + 3] = x.w;
+            for (int i = 0; i < 8; i++)
+                x[i] = live[i] ? __ldg(reinterpret_cast<const uint4 *>(g < 2 * NV ? ql[i] + g * 64 : qr[i])) : make_uint4(0, 0, 0, 0);
+        };
+#pragma unroll
+        for (int p = 0; p < D; p++) load(p, xs[p]);
+#pragma unroll
+        for (int p = 0; p < NC; p++) {
+            uint4 (&x)[8] = xs[p % D];
+            uint8_t *dst = sq + (p < NQ ? 0 : p - NQ) * MLA_QCHUNK + (r >> 5) * 4096;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int k = (lane >> 3) + 4 * i;   // row of the warp's 32
+                *reinterpret_cast<uint4 *>(dst + (k >> 3) * 1024 + (k & 7) * 128 + (u ^ (k & 7)) * 16) =
+                    make_uint4(x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip);
             }
-            if (p < nq) {
-                tmem_st32(tmem + q_col(p), u);
-            } else {
-                uint8_t *dst = sq + (p - nq) * MLA_QCHUNK + (r >> 3) * 1024 + (r & 7) * 128;
+            if (p + D < NC) load(p + D, x);
+            if (p < NQ) {
+                __syncwarp();
+                uint32_t v[32];
+                const uint8_t *src = dst + (lane >> 3) * 1024 + (lane & 7) * 128;
 #pragma unroll
-                for (int k = 0; k < 8; k++)
-                    *reinterpret_cast<uint4 *>(dst + (k ^ (r & 7)) * 16) = make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]);
+                for (int k = 0; k < 8; k++) {
+                    const uint4 y = *reinterpret_cast<const uint4 *>(src + (k ^ (lane & 7)) * 16);
+                    v[4 * k] = y.x, v[4 * k + 1] = y.y, v[4 * k + 2] = y.z, v[4 * k + 3] = y.w;
+                }
+                tmem_st32(tmem + q_col(p), v);
+                __syncwarp();
             }
         }
         tmem_wait_st();
@@ -541,8 +640,8 @@ struct MlaKernel {
         asm volatile("bar.sync 1, 128;" ::: "memory");
         const uint32_t top = BF16 ? 0x7F80u : 0x7C00u;
         bool bad = false;
-        for (int p = 0; p < nv; p++) {
-            const uint4 *src = reinterpret_cast<const uint4 *>(ring_b + (st * nv + p) * MLA_CHUNK + r * 128 + h * 64);
+        for (int p = 0; p < NV; p++) {
+            const uint4 *src = reinterpret_cast<const uint4 *>(ring_b + (st * NV + p) * MLA_CHUNK + r * 128 + h * 64);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const uint4 x = src[k];
@@ -554,10 +653,10 @@ struct MlaKernel {
         bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 1) != 0;
         if (bad) {
             if (h == 0) atomicOr(reinterpret_cast<unsigned long long *>(&c->nonfinite[par]), 1ull << r);
-            for (int p = 0; p < nv; p++)
+            for (int p = 0; p < NV; p++)
 #pragma unroll
                 for (int k = 0; k < 4; k++)
-                    reinterpret_cast<uint4 *>(ring_b + (st * nv + p) * MLA_CHUNK + r * 128 + h * 64)[k] = make_uint4(0, 0, 0, 0);
+                    reinterpret_cast<uint4 *>(ring_b + (st * NV + p) * MLA_CHUNK + r * 128 + h * 64)[k] = make_uint4(0, 0, 0, 0);
         }
         fence_async_smem();
         __syncwarp();
@@ -566,7 +665,7 @@ struct MlaKernel {
     }
 
     __device__ __forceinline__ void store_out(uint32_t tmem, bool live, int64_t token, int head, float ref, float l) {
-        const int half_cols = kv.latent / 2;
+        constexpr int half_cols = 64 * NV;
         const float f = l == 0.0f ? 0.0f : 1.0f / l;
         __half *out = reinterpret_cast<__half *>(q.out) + token * q.ot + head * q.oh + half * half_cols;
         for (int col = 0; col < half_cols; col += 32) {
@@ -588,7 +687,7 @@ struct MlaKernel {
     }
 
     __device__ __forceinline__ void store_piece(uint32_t tmem, const MlaSeg &g, const MlaWalk &w, bool live, int r, float ref, float l) {
-        const int L = kv.latent, half_cols = L / 2;
+        const int L = 128 * NV, half_cols = 64 * NV;
         const int slot = 2 * pair + (g.tile0 == 0);
         float *o = ws.o + ((size_t)slot * L + half * half_cols) * MLA_M + r;
         for (int col = 0; col < half_cols; col += 32) {
@@ -606,22 +705,24 @@ struct MlaKernel {
     }
 };
 
-template <bool BF16, bool FP8>
+template <bool BF16, bool FP8, int NV>
 __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
     k_mla(MoeKvDev kv, MlaSeqAt seq_at, MoeMlaQuery q, const __grid_constant__ CUtensorMap tm, void *ws, int *error) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    const int L = kv.latent, nv = L / 128, nc = 2 * nv + 1, nq = mla_q_tm(L);
+    using K = MlaKernel<BF16, FP8, NV>;
     const int pairs = gridDim.x / 2;
-    uint8_t *ring_b = base, *ring_a = ring_b + MLA_SB * nv * MLA_CHUNK, *sq = ring_a + MLA_RA * MLA_CHUNK;
-    MlaCtl *c = reinterpret_cast<MlaCtl *>(sq + (nc - nq) * MLA_QCHUNK);
+    uint8_t *ring_b = base, *ring_a = ring_b + MLA_SB * NV * MLA_CHUNK, *sq = ring_a + MLA_RA * MLA_CHUNK;
+    MlaCtl *c = reinterpret_cast<MlaCtl *>(sq + mla_q_sm(128 * NV) * MLA_QCHUNK);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int PROD = FP8 ? 8 : 1;
     if (tid == 0) {
         for (int i = 0; i < MLA_RA; i++) tc_mbar_init(&c->full_a[i], PROD), tc_mbar_init(&c->empty_a[i], 1);
         for (int i = 0; i < MLA_SB; i++) tc_mbar_init(&c->full_b[i], PROD), tc_mbar_init(&c->empty_b[i], 1);
-        tc_mbar_init(&c->s_full, 1), tc_mbar_init(&c->s_empty, 4), tc_mbar_init(&c->p_full, 4);
-        tc_mbar_init(&c->pv_done, 1), tc_mbar_init(&c->q_ready, 4), tc_mbar_init(&c->drain, 1);
+        tc_mbar_init(&c->s_full[0], 1), tc_mbar_init(&c->s_full[1], 1);
+        tc_mbar_init(&c->p_full[0], 4), tc_mbar_init(&c->p_full[1], 4);
+        tc_mbar_init(&c->pv_done[0], 1), tc_mbar_init(&c->pv_done[1], 1);
+        tc_mbar_init(&c->q_ready, 4), tc_mbar_init(&c->drain, 1);
         c->dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -665,8 +766,7 @@ __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    MlaKernel<BF16, FP8> k{kv, seq_at, q, &tm, mla_ws(ws, L, pairs), error, ring_b, ring_a, sq, c,
-                           (int)(blockIdx.x & 1), pair, pairs, nv, nc, nq, lane, warp};
+    K k{kv, seq_at, q, &tm, mla_ws(ws, 128 * NV, pairs), error, ring_b, ring_a, sq, c, (int)(blockIdx.x & 1), pair, lane, warp};
     if (k.half == 0 && warp == 3 && lane == 0) {
         // the unit that this pair begins and another one ends (k_mla_join); every call writes the entry
         MlaWalk w = k.walk();
@@ -691,85 +791,148 @@ __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
 }
 
 // ---------------------------------------------------------------------------
-// Joins the pieces of the unit that pair blockIdx.x began and did not end: per
-// row the pieces' sums, each times 2^(its reference - the largest), in the
-// order of the pairs (the same bits every time).  One thread per (row, 8
-// columns, quarter of the pieces); the quarters meet in shared memory.
+// Joins the pieces of cut units: per row the pieces' sums, each times
+// 2^(its reference - the largest), in the order of the pairs (the same bits
+// every time).  Every CTA reads the pairs' entries, so that the columns of the
+// units that were cut (one for a single long sequence, up to one per pair)
+// spread over the whole grid: 4 to 64 columns of a unit per CTA, each thread
+// one row and a quarter of them.
 // ---------------------------------------------------------------------------
-constexpr int MJ_COLS = 8, MJ_PARTS = 4;
+constexpr int MLA_PAIRS = 256;   // CTA pairs at most
+static_assert(MLA_PAIRS <= 4 * MLA_M, "a thread of the join per pair");
+constexpr int MJ_THREADS = 4 * MLA_M;
 
-template <bool BF16>
-__global__ void __launch_bounds__(MLA_M *MJ_PARTS) k_mla_join(MoeKvDev kv, MlaSeqAt seq_at, MoeMlaQuery q, void *wsp, int pairs) {
-    __shared__ float acc[MJ_PARTS][MJ_COLS + 1][MLA_M];
-    moe_pdl_wait();
-    const MlaWs ws = mla_ws(wsp, kv.latent, pairs);
-    const int p = blockIdx.x, r = threadIdx.x % MLA_M, part = threadIdx.x / MLA_M;
-    const MlaWs::Tail t = ws.tail[p];
-    if (!t.on) return;
-    const MlaSeq s = seq_at(t.seq);
-    const int64_t row = (int64_t)t.block * MLA_M + r;
-    const bool live = row < (int64_t)s.n * q.n_heads;
-    const int L = kv.latent, col = blockIdx.y * MJ_COLS, pieces = t.last - p + 1;
-    // piece 0 is this pair's second slot, piece k > 0 pair p + k's first
-    auto slot = [&](int k) { return k == 0 ? 2 * p + 1 : 2 * (p + k); };
-    float m = -INFINITY;
-    if (live)
-#pragma unroll 8
-        for (int k = 0; k < pieces; k++) m = fmaxf(m, ws.ml[(size_t)slot(k) * 2 * MLA_M + r]);
-    const float m0 = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, o[MJ_COLS] = {};
-    const int k0 = pieces * part / MJ_PARTS, k1 = pieces * (part + 1) / MJ_PARTS;
-    if (live)
-#pragma unroll 4
-        for (int k = k0; k < k1; k++) {
-            const float *ml = ws.ml + (size_t)slot(k) * 2 * MLA_M + r;
-            const float f = ex2(ml[0] - m0);
-            const float *src = ws.o + ((size_t)slot(k) * L + col) * MLA_M + r;
-            l = fmaf(f, ml[MLA_M], l);
+// columns col .. col + W - 1 of a thread's row over all pieces, U pieces' loads in flight
+template <int W, int U, typename S>
+__device__ __forceinline__ void join_columns(const float *o, const float *sw, int r, int pieces, size_t stride, S &&slot, float (&sum)[W]) {
+    for (int k0 = 0; k0 < pieces; k0 += U) {
+        float v[U][W], g[U];
 #pragma unroll
-            for (int j = 0; j < MJ_COLS; j++) o[j] = fmaf(f, src[j * MLA_M], o[j]);
+        for (int k = 0; k < U; k++) {
+            const bool in = k0 + k < pieces;
+            const float *src = o + slot(in ? k0 + k : 0) * stride;
+            g[k] = in ? sw[(k0 + k) * MLA_M + r] : 0.0f;
+#pragma unroll
+            for (int j = 0; j < W; j++) v[k][j] = in ? src[j * MLA_M] : 0.0f;
         }
 #pragma unroll
-    for (int j = 0; j < MJ_COLS; j++) acc[part][j][r] = o[j];
-    acc[part][MJ_COLS][r] = l;
-    __syncthreads();
-    if (part || !live) return;
+        for (int k = 0; k < U; k++)
 #pragma unroll
-    for (int k = 1; k < MJ_PARTS; k++) {
-        l += acc[k][MJ_COLS][r];
-#pragma unroll
-        for (int j = 0; j < MJ_COLS; j++) o[j] += acc[k][j][r];
+            for (int j = 0; j < W; j++) sum[j] = fmaf(g[k], v[k][j], sum[j]);
     }
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    const int64_t token = s.q0 + row / q.n_heads, head = row % q.n_heads;
-    uint4 x;
-    x.x = pack2<BF16>(o[0] * f, o[1] * f);
-    x.y = pack2<BF16>(o[2] * f, o[3] * f);
-    x.z = pack2<BF16>(o[4] * f, o[5] * f);
-    x.w = pack2<BF16>(o[6] * f, o[7] * f);
-    *reinterpret_cast<uint4 *>(reinterpret_cast<__half *>(q.out) + token * q.ot + head * q.oh + col) = x;
-    if (col == 0 && q.lse) q.lse[token * q.n_heads + head] = l == 0.0f ? -INFINITY : m * 0.69314718055994531f + logf(l);
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(MJ_THREADS, 2) k_mla_join(MoeKvDev kv, MlaSeqAt seq_at, MoeMlaQuery q, void *wsp, int pairs) {
+    extern __shared__ float sw[];   // [pieces][128] references, then factors
+    __shared__ float sl[4][MLA_M];
+    __shared__ int on[MLA_PAIRS], units[MLA_PAIRS], n_units;
+    moe_pdl_wait();
+    const MlaWs ws = mla_ws(wsp, kv.latent, pairs);
+    const int r = threadIdx.x % MLA_M, part = threadIdx.x / MLA_M, L = kv.latent;
+    const int me = threadIdx.x;
+    if (me < pairs) on[me] = ws.tail[me].on;
+    __syncthreads();
+    if (me < pairs) {   // the pairs that begin a cut unit, in order
+        int rank = 0;
+        for (int j = 0; j < me; j++) rank += on[j];
+        if (on[me]) units[rank] = me;
+        if (me == pairs - 1) n_units = rank + on[me];
+    }
+    __syncthreads();
+    const int n = n_units;
+    int cols = 4;   // of an item: as few as give each CTA one
+    while (cols < 64 && n * (L / cols) > (int)gridDim.x) cols <<= 1;
+    const int per = L / cols, items = n * per;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const int p = units[item / per], col0 = (item % per) * cols;
+        const MlaWs::Tail t = ws.tail[p];
+        const MlaSeq s = seq_at(t.seq);
+        const uint32_t row = (uint32_t)t.block * MLA_M + r;
+        const bool live = row < (uint32_t)s.n * q.n_heads;
+        const int pieces = t.last - p + 1;
+        // piece 0 is this pair's second slot, piece k > 0 pair p + k's first
+        auto slot = [&](int k) { return (size_t)(k == 0 ? 2 * p + 1 : 2 * (p + k)); };
+        __syncthreads();
+#pragma unroll 8
+        for (int k = part; k < pieces; k += 4) sw[k * MLA_M + r] = live ? ws.ml[slot(k) * 2 * MLA_M + r] : -INFINITY;
+        __syncthreads();
+        float m = -INFINITY;
+#pragma unroll 8
+        for (int k = 0; k < pieces; k++) m = fmaxf(m, sw[k * MLA_M + r]);
+        const float m0 = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f;
+        __syncthreads();
+#pragma unroll 8
+        for (int k = part; k < pieces; k += 4) {
+            const float f = ex2(sw[k * MLA_M + r] - m0);
+            sw[k * MLA_M + r] = f;
+            if (live) l = fmaf(f, ws.ml[slot(k) * 2 * MLA_M + MLA_M + r], l);
+        }
+        sl[part][r] = l;
+        __syncthreads();
+        l = (sl[0][r] + sl[1][r]) + (sl[2][r] + sl[3][r]);
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+        const int64_t token = s.q0 + row / (uint32_t)q.n_heads, head = row % (uint32_t)q.n_heads;
+        if (live) {
+            const int mine = cols / 4;   // 1, 2, 4, 8 or 16
+            __half *out = reinterpret_cast<__half *>(q.out) + token * q.ot + head * q.oh;
+            const size_t stride = (size_t)L * MLA_M;
+            for (int c0 = 0; c0 < mine; c0 += 4) {
+                const int col = col0 + part * mine + c0;
+                const float *o = ws.o + (size_t)col * MLA_M + r;
+                if (mine >= 4) {
+                    float a[4] = {};
+                    if (pieces <= 4) join_columns<4, 4>(o, sw, r, pieces, stride, slot, a);
+                    else join_columns<4, 8>(o, sw, r, pieces, stride, slot, a);
+                    *reinterpret_cast<uint2 *>(out + col) = make_uint2(pack2<BF16>(a[0] * f, a[1] * f), pack2<BF16>(a[2] * f, a[3] * f));
+                } else if (mine == 2) {
+                    float a[2] = {};
+                    join_columns<2, 16>(o, sw, r, pieces, stride, slot, a);
+                    *reinterpret_cast<uint32_t *>(out + col) = pack2<BF16>(a[0] * f, a[1] * f);
+                } else {
+                    float a[1] = {};
+                    join_columns<1, 25>(o, sw, r, pieces, stride, slot, a);
+                    *reinterpret_cast<uint16_t *>(out + col) = (uint16_t)pack2<BF16>(a[0] * f, 0.0f);
+                }
+            }
+            if (col0 == 0 && part == 0 && q.lse)
+                q.lse[token * q.n_heads + head] = l == 0.0f ? -INFINITY : m * 0.69314718055994531f + logf(l);
+        }
+    }
 }
 
 size_t mla_smem(int latent) {
-    const int nv = latent / 128, nc = 2 * nv + 1;
-    return 1024 + (size_t)(MLA_SB * nv + MLA_RA) * MLA_CHUNK + (size_t)(nc - mla_q_tm(latent)) * MLA_QCHUNK + sizeof(MlaCtl);
+    const int nv = latent / 128;
+    return 1024 + (size_t)(MLA_SB * nv + MLA_RA) * MLA_CHUNK + (size_t)mla_q_sm(latent) * MLA_QCHUNK + sizeof(MlaCtl);
 }
 
-template <bool BF16, bool FP8>
+template <bool BF16, bool FP8, int NV>
 void launch(const MoeKvDev &kv, const MlaSeqAt &at, const MoeMlaQuery &q, const CUtensorMap &tm, void *ws, int pairs,
             int *error, cudaStream_t s) {
     static size_t done[MOE_MAX_DEVICES];
     const size_t smem = mla_smem(kv.latent);
-    moe_smem_limit(k_mla<BF16, FP8>, smem, done);
-    moe_launch_pdl(k_mla<BF16, FP8>, dim3(2 * pairs), dim3(FP8 ? 512 : 256), smem, s, kv, at, q, tm, ws, error);
-    moe_launch_pdl(k_mla_join<BF16>, dim3(pairs, kv.latent / MJ_COLS), dim3(MLA_M * MJ_PARTS), 0, s, kv, at, q, ws, pairs);
+    moe_smem_limit(k_mla<BF16, FP8, NV>, smem, done);
+    moe_launch_pdl(k_mla<BF16, FP8, NV>, dim3(2 * pairs), dim3(FP8 ? 512 : 256), smem, s, kv, at, q, tm, ws, error);
+    moe_launch_pdl(k_mla_join<BF16>, dim3(4 * pairs), dim3(MJ_THREADS), sizeof(float) * pairs * MLA_M, s, kv, at, q, ws, pairs);
 }
+
+template <bool BF16, bool FP8, typename... A>
+void by_latent(const MoeKvDev &kv, A &&...a) {
+    switch (kv.latent) {
+        case 128: launch<BF16, FP8, 1>(kv, a...); break;
+        case 256: launch<BF16, FP8, 2>(kv, a...); break;
+        case 384: launch<BF16, FP8, 3>(kv, a...); break;
+        default: launch<BF16, FP8, 4>(kv, a...);
+    }
+}
+
+int mla_pairs(int sms) { return sms / 2 < 1 ? 1 : sms / 2 > MLA_PAIRS ? MLA_PAIRS : sms / 2; }
 
 }  // namespace
 
 size_t moe_mla_ws_bytes(int latent, int sms) {
-    const int pairs = sms / 2;
+    const int pairs = mla_pairs(sms);
     return ((size_t)pairs * sizeof(MlaWs::Tail) + 255) / 256 * 256 + (size_t)pairs * 2 * (2 + latent) * MLA_M * sizeof(float);
 }
 
@@ -782,10 +945,10 @@ int moe_launch_mla(const MoeKvDev &kv, const MoeKvBatchDev &b, const MoeMlaQuery
                                        kv.page_shift >= 6 ? MLA_N : 1u << kv.page_shift))
         return -1;
     switch (kv.format) {
-        case MOE_KV_F16: launch<false, false>(kv, at, q, tm, ws, sms / 2, error, s); break;
-        case MOE_KV_BF16: launch<true, false>(kv, at, q, tm, ws, sms / 2, error, s); break;
-        case MOE_KV_FP8_F16: launch<false, true>(kv, at, q, tm, ws, sms / 2, error, s); break;
-        default: launch<true, true>(kv, at, q, tm, ws, sms / 2, error, s);
+        case MOE_KV_F16: by_latent<false, false>(kv, at, q, tm, ws, mla_pairs(sms), error, s); break;
+        case MOE_KV_BF16: by_latent<true, false>(kv, at, q, tm, ws, mla_pairs(sms), error, s); break;
+        case MOE_KV_FP8_F16: by_latent<false, true>(kv, at, q, tm, ws, mla_pairs(sms), error, s); break;
+        default: by_latent<true, true>(kv, at, q, tm, ws, mla_pairs(sms), error, s);
     }
     LAUNCH_COUNT(launches);
     LAUNCH_COUNT(launches);

@@ -256,6 +256,17 @@ __device__ __forceinline__ bool tc_wait(uint64_t *b, uint32_t parity) {
         if (clock64() - t0 > TC_WAIT_CYCLES) return false;
     }
 }
+// one look at a phase, without waiting
+__device__ __forceinline__ uint32_t tc_test(uint64_t *b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(umma_smem_u32(b)), "r"(parity)
+        : "memory");
+    return ok;
+}
 // after a producer gave up: wait (bounded) for the copies it issued into
 // the last `ns` stages of a ring, so that none lands after the CTA exits
 __device__ __forceinline__ void tc_drain(uint64_t *full, int issued, int ns) {
