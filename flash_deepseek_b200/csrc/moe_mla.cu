@@ -44,8 +44,11 @@ constexpr int MLA_QCHUNK = MLA_M * 128;     // bytes of a 128-row x 64-value que
 constexpr int MLA_RA = 6;                   // chunks of ring A
 constexpr int MLA_SB = 3;                   // tiles of ring B
 // Tensor-memory columns: the output from 0 (at most 256), two score tiles of 64 (the weights of a tile, 32 columns of
-// 16-bit pairs, take the place of its scores), the query's chunks.
-constexpr int MLA_TM_S = 256, MLA_TM_Q = 384;
+// 16-bit pairs, take the place of its second half), the query's chunks.
+constexpr int MLA_TM_S = 256, MLA_TM_P = 32, MLA_TM_Q = 384;
+#ifndef MLA_XW
+#define MLA_XW 8                            // warps that expand the 8-bit formats (8 or 4)
+#endif
 constexpr float MLA_RAISE = 8.0f;           // log2: how far scores may pass the reference before it is raised
 
 // Tensor memory left for query chunks of 32 columns (64 values) each: all of
@@ -55,17 +58,23 @@ __host__ __device__ constexpr int mla_q_tm(int latent) {
     return all < fit ? all : fit;
 }
 
-// Query chunks in shared memory: the others, one at least (the way of all into tensor memory)
+// Query chunks in shared memory: the others, or room for those on their way into tensor memory
 __host__ __device__ constexpr int mla_q_sm(int latent) {
-    const int rest = latent / 64 + 1 - mla_q_tm(latent);
-    return rest > 1 ? rest : 1;
+    const int tm = mla_q_tm(latent), rest = latent / 64 + 1 - tm;
+    return rest > tm ? rest : tm;
 }
 
 struct MlaCtl {   // control block behind the tiles
     uint64_t full_a[MLA_RA], empty_a[MLA_RA], full_b[MLA_SB], empty_b[MLA_SB];   // chunks of ring A, tiles of ring B
+    uint64_t full_r[2], empty_r[2];   // 8-bit formats: rotary chunks by tile parity
     uint64_t s_full[2], p_full[2], pv_done[2], q_ready, drain;   // by tile parity
     uint64_t nonfinite[2];       // by tile parity: rows of a tile with an infinity or a NaN in this CTA's latent half
-    uint8_t valid[MLA_SB][8];    // 8-row groups of a tile whose page exists
+    struct Rows {                // each softmax warp's walk over the segments (in registers it would cost them 30)
+        MlaWalk w;
+        MlaSeg g;
+        int more;
+    } rows[4];
+    uint8_t valid[4][8];         // by tile: 8-row groups whose page exists
     int64_t w0, w1, off0;        // the pair's share: first and last tile, place of the first in its sequence
     int64_t scan[32];
     int64_t total;
@@ -101,6 +110,15 @@ struct MlaSeqAt {
                        (int64_t)b.pages_per_seq << page_shift);
     }
 };
+
+// The warp waits for a phase (tc_wait_warp); the polling is out of line: the
+// loops of this kernel's roles share one instruction cache of some 32 KB, and
+// with everything unrolled and inlined a fifth to a third of the fetches missed
+// it, which cost more than any other stall.
+__device__ __noinline__ bool poll(uint64_t *b, uint32_t parity) { return tc_wait_warp(b, parity); }
+__device__ __forceinline__ bool wait_phase(uint64_t *b, uint32_t parity) {
+    return __all_sync(0xffffffffu, tc_test(b, parity)) || poll(b, parity);
+}
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -139,18 +157,18 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // 4 e4m3 codes times a group's scale as 4 16-bit values.  The code's exponent
 // and mantissa bits placed in the 16-bit format's fields are the value over
 // 2^120 (bf16) or 2^8 (fp16), subnormals too; f holds 2^(120 + k) or 2^(8 + k).
+// Each half word holds a code: shifted up by a product, then the sign (bit 11 or
+// 14) moved to bit 15 by adding 15 times or once itself; products and sums run
+// on another pipe than the byte permutes and masks, which bound this.
 template <bool BF16>
 __device__ __forceinline__ uint2 expand4(uint32_t w, uint32_t f) {
-    const uint32_t lo = __byte_perm(w, 0, 0x1404), hi = __byte_perm(w, 0, 0x3424);
-    uint2 r;
+    constexpr uint32_t up = BF16 ? 16 : 128, sign = BF16 ? 0x08000800u : 0x40004000u, times = BF16 ? 15 : 1;
+    const uint32_t lo = __byte_perm(w, 0, 0x4140) * up, hi = __byte_perm(w, 0, 0x4342) * up;
+    uint2 r = make_uint2((lo & sign) * times + lo, (hi & sign) * times + hi);
     if (BF16) {
-        r.x = (lo & 0x80008000u) | ((lo & 0x7F007F00u) >> 4);
-        r.y = (hi & 0x80008000u) | ((hi & 0x7F007F00u) >> 4);
         asm("mul.bf16x2 %0, %0, %1;" : "+r"(r.x) : "r"(f));
         asm("mul.bf16x2 %0, %0, %1;" : "+r"(r.y) : "r"(f));
     } else {
-        r.x = (lo & 0x80008000u) | ((lo & 0x7F007F00u) >> 1);
-        r.y = (hi & 0x80008000u) | ((hi & 0x7F007F00u) >> 1);
         asm("mul.f16x2 %0, %0, %1;" : "+r"(r.x) : "r"(f));
         asm("mul.f16x2 %0, %0, %1;" : "+r"(r.y) : "r"(f));
     }
@@ -197,7 +215,7 @@ struct MlaKernel {
     const CUtensorMap *tm;
     MlaWs ws;
     int *error;
-    uint8_t *ring_b, *ring_a, *sq;
+    uint8_t *ring_b, *ring_a, *ring_r, *sq;
     MlaCtl *c;
     int half, pair;
     int lane, warp;
@@ -223,13 +241,14 @@ struct MlaKernel {
     }
 
     // after a wait gave up: none of the copies issued so far may land after the CTA has ended
-    __device__ void stop_tma(int ia, int ib) {
+    __device__ void stop_tma(int ia, int ib, int ir) {
         give_up();
+        if (FP8) return tc_drain(c->full_r, ir, 2);
         tc_drain(c->full_a, ia, MLA_RA);
         tc_drain(c->full_b, ib, MLA_SB);
     }
 
-    // ---- loads, 16-bit formats: lane j < 8 handles rows 8 j .. of a tile
+    // ---- TMA: lane j < 8 handles rows 8 j .. of a tile.  16-bit formats: all chunks; 8-bit formats: the rotary one.
     __device__ void produce_tma() {
         MlaWalk w = walk();
         MlaSeg g;
@@ -249,17 +268,30 @@ struct MlaKernel {
                 }
                 const bool box = lane < 8 && (lane * 8) % rows_box == 0;
                 const int off = lane * 8 * 128;
-                if (!tc_wait_warp(&c->empty_b[st], (ib / MLA_SB + 1) & 1)) return stop_tma(ia, ib);
-                if (lane < 8) c->valid[st][lane] = ok;
+                if (FP8) {
+                    // valid[] of tile ib - 4 is read: its output product was issued before the scores of tile ib - 2
+                    const int sr = ib & 1;
+                    if (!wait_phase(&c->empty_r[sr], (ib / 2 + 1) & 1)) return stop_tma(0, 0, ib);
+                    if (lane < 8) c->valid[ib & 3][lane] = ok;
+                    __syncwarp();
+                    if (lane == 0) tc_expect(&c->full_r[sr], MLA_CHUNK);
+                    __syncwarp();
+                    if (box) tc_tma2(ring_r + sr * MLA_CHUNK + off, tm, 64 * NV, row, &c->full_r[sr]);   // 16-bit units
+                    continue;
+                }
+                if (!wait_phase(&c->empty_b[st], (ib / MLA_SB + 1) & 1)) return stop_tma(ia, ib, 0);
+                if (lane < 8) c->valid[ib & 3][lane] = ok;
                 __syncwarp();
                 if (lane == 0) tc_expect(&c->full_b[st], (uint32_t)NV * MLA_CHUNK);
                 __syncwarp();
                 if (box)
+#pragma unroll 1
                     for (int p = 0; p < NV; p++)
                         tc_tma2(ring_b + (st * NV + p) * MLA_CHUNK + off, tm, chunk_at(p) * 64, row, &c->full_b[st]);
+#pragma unroll 1
                 for (int p = NV; p < NC; p++, ia++) {
                     const int sa = ia % MLA_RA;
-                    if (!tc_wait_warp(&c->empty_a[sa], (ia / MLA_RA + 1) & 1)) return stop_tma(ia, ib + 1);
+                    if (!wait_phase(&c->empty_a[sa], (ia / MLA_RA + 1) & 1)) return stop_tma(ia, ib + 1, 0);
                     if (lane == 0) tc_expect(&c->full_a[sa], MLA_CHUNK);
                     __syncwarp();
                     if (box) tc_tma2(ring_a + sa * MLA_CHUNK + off, tm, chunk_at(p) * 64, row, &c->full_a[sa]);
@@ -268,99 +300,112 @@ struct MlaKernel {
         }
     }
 
-    // ---- loads, 8-bit formats: 8 warps, 4 threads per row, 16 codes of every chunk each.  The next tile's
-    // loads are issued as this tile's chunks are expanded, so a tile's bytes are always in flight.
-    __device__ void produce_expand() {
-        constexpr int L = 128 * NV;
-        const int tid = threadIdx.x - 256, r = tid >> 2, qd = tid & 3;
-        MlaWalk w = walk();
+    // ---- 8-bit formats: 4 warps expand the chunks of this CTA's half into ring B, 4 threads per row, 16 codes of a chunk
+    // each; from there they are copied into ring A of the other CTA, whose scores need them too.  So each CTA reads and
+    // expands half of a row.  Codes are loaded a tile ahead, page numbers two.
+    struct Cursor {   // a place in the pair's tiles
+        MlaWalk w;
         MlaSeg g;
-        int ia = 0, ib = 0;
-        uint4 code[2 * NV], rope[2], sc;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        // loads of tile t of the current segment
-        const uint8_t *row;
-        bool ok;
-        auto locate = [&](int seq, const MlaSeq &s, int t) {
-            const long long f = flat(seq, s, (int64_t)t * MLA_N + r);
-            ok = f >= 0;
-            if (f == -1) kv_error(error, KV_ERR_BATCH);
-            row = ok ? kv.data + f * kv.row_bytes : nullptr;
+        int t;
+        bool more;
+    };
+    __device__ __forceinline__ void step(Cursor &u) {
+        if (u.more && ++u.t >= u.g.tile1) {
+            u.more = u.w.next(u.g, seq_at);
+            u.t = u.g.tile0;
+        }
+    }
+    // the page of this thread's row of the cursor's tile (-1: none, -2: behind the sequence)
+    __device__ __forceinline__ int page_of(const Cursor &u, int r, int &in_page) {
+        const int64_t pos = (int64_t)u.t * MLA_N + r;
+        in_page = (int)(pos & ((1 << kv.page_shift) - 1));
+        if (!u.more || pos >= u.w.s.len) return -2;
+        const int64_t pi = pos >> kv.page_shift;
+        return pi < seq_at.b.pages_per_seq ? __ldg(seq_at.b.pages + (size_t)u.g.seq * seq_at.b.pages_per_seq + pi) : -1;
+    }
+    __device__ __forceinline__ const uint8_t *row_of(int page, int in_page) {
+        // (a page out of range: the TMA warp reports it and hides the row)
+        return page < 0 || page >= kv.n_pages ? nullptr : kv.data + (((int64_t)page << kv.page_shift) + in_page) * kv.row_bytes;
+    }
+    __device__ void produce_expand() {
+        constexpr int L = 128 * NV, RT = 8 / MLA_XW;   // rows of a thread: r, and r + 32
+        const int tid = threadIdx.x - 256, r = tid >> 2, qd = tid & 3;
+        const int n = (int)(c->w1 - c->w0);
+        const uint32_t sw = (uint32_t)(r & 7), at = (uint32_t)(r >> 3) * 1024 + sw * 128;
+        const uint32_t lo_at = at + ((2 * qd) ^ sw) * 16, hi_at = at + ((2 * qd + 1) ^ sw) * 16;
+        const int code_at = half * NV * 64 + qd * 16, scale_at = L + 2 * MOE_KV_ROPE + half * NV * 2 + (qd >> 1);
+        uint4 code[RT][NV];
+        uint32_t sb[RT][NV];
+        auto load = [&](const uint8_t *row, int p, uint4 &v, uint32_t &b) {
+            v = row ? __ldg(reinterpret_cast<const uint4 *>(row + code_at + p * 64)) : make_uint4(0, 0, 0, 0);
+            b = row ? __ldg(row + scale_at + p * 2) : 127u;
         };
-        auto load_sc = [&]() {
-            sc = zero;
-            if (!row) return;
-            const uint32_t *p = reinterpret_cast<const uint32_t *>(row + L + 2 * MOE_KV_ROPE);
-            sc.x = __ldg(p);
-            if (L > 128) sc.y = __ldg(p + 1);
-            if (L > 256) sc.z = __ldg(p + 2);
-            if (L > 384) sc.w = __ldg(p + 3);
+        Cursor u{walk(), MlaSeg{}, 0, true};
+        u.more = u.w.next(u.g, seq_at);
+        u.t = u.g.tile0;
+        int page[RT], in_page[RT];
+        auto look = [&]() {
+#pragma unroll
+            for (int k = 0; k < RT; k++) page[k] = page_of(u, r + 32 * k, in_page[k]);
         };
-        auto load_code = [&](int p) { return row ? __ldg(reinterpret_cast<const uint4 *>(row + chunk_at(p) * 64) + qd) : zero; };
-        auto load_rope = [&](int k) { return row ? __ldg(reinterpret_cast<const uint4 *>(row + L) + 2 * qd + k) : zero; };
-        if (!w.next(g, seq_at)) return;
-        int t = g.tile0;
-        locate(g.seq, w.s, t);
-        load_sc();
+        look();
 #pragma unroll
-        for (int p = 0; p < 2 * NV; p++) code[p] = load_code(p);
-        rope[0] = load_rope(0), rope[1] = load_rope(1);
-        for (bool more = true; more; ib++) {
-            const int st = ib % MLA_SB;
-            const bool cur_ok = ok;
-            const uint4 s4 = sc;
-            // the next tile
-            if (++t >= g.tile1) {
-                more = w.next(g, seq_at);
-                t = g.tile0;
-            }
-            if (more) {
-                locate(g.seq, w.s, t);
-                load_sc();
-            } else {
-                row = nullptr;
-            }
-            if (!tc_wait_warp(&c->empty_b[st], (ib / MLA_SB + 1) & 1)) return give_up();
-            if (lane == 0) c->valid[st][warp - 8] = cur_ok;   // a warp holds the 8 rows of one group
-            const uint32_t sw = (uint32_t)(r & 7);
-            const uint32_t at = (uint32_t)(r >> 3) * 1024 + sw * 128;
+        for (int k = 0; k < RT; k++) {
+            const uint8_t *row = row_of(page[k], in_page[k]);
 #pragma unroll
-            for (int p = 0; p < NC; p++) {
-                uint8_t *dst;
-                if (p < NV) dst = ring_b + (st * NV + p) * MLA_CHUNK;
-                else {
-                    const int sa = ia % MLA_RA;
-                    if (!tc_wait_warp(&c->empty_a[sa], (ia / MLA_RA + 1) & 1)) return give_up();
-                    dst = ring_a + sa * MLA_CHUNK;
-                }
-                uint4 lo, hi;
-                if (p < 2 * NV) {
-                    const uint4 v = code[p < 2 * NV ? p : 0];
-                    const int grp = 2 * chunk_at(p) + (qd >> 1);
-                    const uint32_t word = grp < 4 ? s4.x : grp < 8 ? s4.y : grp < 12 ? s4.z : s4.w;
-                    const uint32_t f = scale2<BF16>(word >> (8 * (grp & 3)) & 255);
+            for (int p = 0; p < NV; p++) load(row, p, code[k][p], sb[k][p]);
+        }
+        step(u);
+        look();
+#pragma unroll 1
+        for (int i = 0; i < n; i++) {
+            const int st = i % MLA_SB;
+            const uint8_t *row[RT];   // of tile i + 1
+#pragma unroll
+            for (int k = 0; k < RT; k++) row[k] = row_of(page[k], in_page[k]);
+            step(u);
+            look();                   // the pages of tile i + 2
+            if (!wait_phase(&c->empty_b[st], (i / MLA_SB + 1) & 1)) return give_up();
+#pragma unroll
+            for (int p = 0; p < NV; p++) {
+#pragma unroll
+                for (int k = 0; k < RT; k++) {
+                    const uint32_t f = scale2<BF16>(sb[k][p]);
+                    const uint4 v = code[k][p];
+                    load(row[k], p, code[k][p], sb[k][p]);
                     const uint2 a = expand4<BF16>(v.x, f), b = expand4<BF16>(v.y, f);
                     const uint2 d = expand4<BF16>(v.z, f), e = expand4<BF16>(v.w, f);
-                    lo = make_uint4(a.x, a.y, b.x, b.y);
-                    hi = make_uint4(d.x, d.y, e.x, e.y);
-                    code[p < 2 * NV ? p : 0] = load_code(p);
-                } else {
-                    lo = rope[0], hi = rope[1];
-                    rope[0] = load_rope(0), rope[1] = load_rope(1);
-                }
-                if (!cur_ok) lo = zero, hi = zero;
-                *reinterpret_cast<uint4 *>(dst + at + ((2 * qd) ^ sw) * 16) = lo;
-                *reinterpret_cast<uint4 *>(dst + at + ((2 * qd + 1) ^ sw) * 16) = hi;
-                fence_async_smem();
-                __syncwarp();
-                if (p >= NV) {
-                    if (lane == 0) tc_arrive(&c->full_a[ia % MLA_RA]);
-                    ia++;
-                } else if (p == NV - 1) {
-                    if (lane == 0) tc_arrive(&c->full_b[st]);
+                    uint8_t *dst = ring_b + (st * NV + p) * MLA_CHUNK + k * 4096;   // 32 rows further
+                    *reinterpret_cast<uint4 *>(dst + lo_at) = make_uint4(a.x, a.y, b.x, b.y);
+                    *reinterpret_cast<uint4 *>(dst + hi_at) = make_uint4(d.x, d.y, e.x, e.y);
                 }
             }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) tc_arrive(&c->full_b[st]);
         }
+    }
+    // One warp copies each expanded chunk to the other CTA once its scores of the tile before are done with the slot
+    // (bulk copies: 16-byte remote stores from the expanding threads took 4500 cycles a tile, against 2700 for the rest).
+    // A stage of ring B is free when its output product is done and the other CTA has used what was copied from it.
+    __device__ void forward() {
+        const int n = (int)(c->w1 - c->w0);
+        const uint32_t other = half ^ 1, ra = cluster_map(ring_a, other), fa = cluster_map(c->full_a, other);
+        for (int i = 0; i < n; i++) {
+            const int st = i % MLA_SB;
+            if (!wait_phase(&c->full_b[st], (i / MLA_SB) & 1)) return stop_forward();
+            for (int p = 0; p < NV; p++) {
+                if (!wait_phase(&c->empty_a[p], (i + 1) & 1)) return stop_forward();
+                if (lane == 0) cluster_copy_async(ra + p * MLA_CHUNK, ring_b + (st * NV + p) * MLA_CHUNK, MLA_CHUNK, fa + p * 8);
+            }
+            if (i > 0 && lane == 0) tc_arrive(&c->empty_b[(i - 1) % MLA_SB]);
+            __syncwarp();
+        }
+    }
+    // after a wait gave up: the copies into the other CTA that are under way land long before it can end
+    __device__ void stop_forward() {
+        give_up();
+        __nanosleep(100000);
     }
 
     // ---- MMA issue: one warp, every lane runs the loop, an elected lane issues.  Operands are broadcast from lane 0
@@ -369,10 +414,10 @@ struct MlaKernel {
     // Barriers are tested ahead, before the MMAs in front of their use: a test of a completed phase takes 100 cycles
     // from issue to branch, which the tensor pipe would stand idle.
     __device__ __forceinline__ bool then_wait(uint32_t seen, uint64_t *b, uint32_t parity) {
-        return __all_sync(0xffffffffu, seen) || tc_wait_warp(b, parity);
+        return __all_sync(0xffffffffu, seen) || poll(b, parity);
     }
     struct Issue {
-        uint32_t tmem, rb, ra, sq;         // base addresses
+        uint32_t tmem, rb, ra, rr, sq;     // base addresses
         int st, sa, phase_b, phase_a;      // next tile's stage and next chunk's slot, their parities
         uint32_t seen_b;                   // the test of the next tile's ring B stage
     };
@@ -382,11 +427,11 @@ struct MlaKernel {
         if (!then_wait(seen, &c->p_full[i & 1], (i >> 1) & 1)) return false;
         x.seen_b = tc_test(&c->full_b[x.st], x.phase_b);
         tmem_fence_after();
-        const uint32_t ts = x.tmem + MLA_TM_S + (i & 1) * 64;
+        const uint32_t ts = x.tmem + MLA_TM_S + (i & 1) * 64 + MLA_TM_P;
         const uint64_t d = umma_desc_sw128_mn(x.rb + st * NV * MLA_CHUNK, MLA_CHUNK);
-#pragma unroll
-        for (int k = 0; k < MLA_N / 16; k++)   // 16 cache rows: 2048 bytes of the tile, 8 columns of weights
-            umma_f16_ta_warp(x.tmem, ts + k * 8, d + k * (2048 >> 4), id, k == 0 ? more : 1u);
+        // four steps of 16 cache rows: 2048 bytes of the tile, 8 columns of weights each
+        static_assert(MLA_N == 64, "four steps");
+        umma_f16_ta_warp4<(2048 >> 4)>(x.tmem, ts, d, id, more);
         umma_commit_warp(&c->empty_b[st]);
         umma_commit_warp(&c->pv_done[i & 1]);
         return true;
@@ -395,33 +440,61 @@ struct MlaKernel {
     __device__ bool scores(Issue &x, int it, uint32_t &seen) {
         constexpr uint32_t id = umma_idesc_16(MLA_M, MLA_N, BF16, 0);
         if (!then_wait(x.seen_b, &c->full_b[x.st], x.phase_b)) return false;
-        uint32_t seen_a = 0;
+        x.seen_b = 0;   // of this tile only: the first tile of a segment has no output() behind it that tests the next
         tmem_fence_after();
-        const uint64_t a0 = umma_desc_sw128(x.sq);
         // The score tile it & 1 is free: its weights' product (tile it - 2) was issued before, and the tensor pipe
         // runs in order
         const uint32_t ts = x.tmem + MLA_TM_S + (it & 1) * 64;
+        uint32_t seen_a = 0;
+        auto chunk_tm = [&](uint32_t q_at, uint32_t k_at, uint32_t first) {   // the query's chunk in tensor memory
+            umma_f16_ta_warp4<2>(ts, q_at, umma_desc_sw128(k_at), id, first);
+        };
+        auto chunk_sm = [&](uint32_t q_at, uint32_t k_at) {                   // in shared memory
+            umma_f16_warp4(ts, umma_desc_sw128(q_at), umma_desc_sw128(k_at), id);
+        };
+        static_assert(NQ >= NV, "the own half's query chunks are in tensor memory");
+        const uint32_t rb = x.rb + x.st * NV * MLA_CHUNK;
 #pragma unroll
-        for (int p = 0; p < NC; p++) {
-            if (p >= NV && !then_wait(seen_a, &c->full_a[x.sa], x.phase_a)) return false;
-            const int sa = x.sa;
-            const uint64_t b = umma_desc_sw128(p < NV ? x.rb + (x.st * NV + p) * MLA_CHUNK : x.ra + sa * MLA_CHUNK);
-            if (p >= NV && ++x.sa == MLA_RA) x.sa = 0, x.phase_a ^= 1;
-            if (p >= NV - 1 && p < NC - 1) seen_a = tc_test(&c->full_a[x.sa], x.phase_a);
-            if (p == NC - 1) seen = tc_test(&c->p_full[(it - 1) & 1], ((it - 1) >> 1) & 1);
+        for (int p = 0; p < NV; p++) {
+            if (p == NV - 1) seen_a = FP8 ? tc_test(&c->full_a[0], it & 1) : tc_test(&c->full_a[x.sa], x.phase_a);
+            chunk_tm(x.tmem + q_col(p), rb + p * MLA_CHUNK, p > 0);
+        }
+        if (FP8) {
+            // ring A: one slot per chunk, filled by the other CTA; armed for the next tile as soon as this one is in
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if (p < NQ) umma_f16_ta_warp(ts, x.tmem + q_col(p) + k * 8, b + k * 2, id, p > 0 || k > 0);
-                else umma_f16_warp(ts, a0 + (p - NQ) * (MLA_QCHUNK >> 4) + k * 2, b + k * 2, id, p > 0 || k > 0);
+            for (int p = NV; p < 2 * NV; p++) {
+                const int sa = p - NV;
+                if (!then_wait(seen_a, &c->full_a[sa], it & 1)) return false;
+                if (lane == 0) tc_expect(&c->full_a[sa], MLA_CHUNK);
+                seen_a = sa + 1 < NV ? tc_test(&c->full_a[sa + 1], it & 1) : tc_test(&c->full_r[it & 1], (it >> 1) & 1);
+                if (p < NQ) chunk_tm(x.tmem + q_col(p), x.ra + sa * MLA_CHUNK, 1u);
+                else chunk_sm(x.sq + (uint32_t)(p - NQ) * MLA_QCHUNK, x.ra + sa * MLA_CHUNK);
+                umma_commit_to_warp(&c->empty_a[sa], (uint16_t)(1u << (half ^ 1)));
             }
-            if (p >= NV) umma_commit_warp(&c->empty_a[sa]);
+            if (!then_wait(seen_a, &c->full_r[it & 1], (it >> 1) & 1)) return false;
+            seen = tc_test(&c->p_full[(it + 1) & 1], (uint32_t)(it - 1) >> 1 & 1);
+            if (2 * NV < NQ) chunk_tm(x.tmem + q_col(2 * NV), x.rr + (it & 1) * MLA_CHUNK, 1u);
+            else chunk_sm(x.sq + (uint32_t)(2 * NV - NQ) * MLA_QCHUNK, x.rr + (it & 1) * MLA_CHUNK);
+            umma_commit_warp(&c->empty_r[it & 1]);
+        } else {
+#pragma unroll
+            for (int p = NV; p < NC; p++) {
+                const int sa = x.sa;
+                if (!then_wait(seen_a, &c->full_a[sa], x.phase_a)) return false;
+                if (++x.sa == MLA_RA) x.sa = 0, x.phase_a ^= 1;
+                if (p < NC - 1) seen_a = tc_test(&c->full_a[x.sa], x.phase_a);
+                else seen = tc_test(&c->p_full[(it + 1) & 1], (uint32_t)(it - 1) >> 1 & 1);
+                if (p < NQ) chunk_tm(x.tmem + q_col(p), x.ra + sa * MLA_CHUNK, 1u);
+                else chunk_sm(x.sq + (uint32_t)(p - NQ) * MLA_QCHUNK, x.ra + sa * MLA_CHUNK);
+                umma_commit_warp(&c->empty_a[sa]);
+            }
         }
         umma_commit_warp(&c->s_full[it & 1]);
         if (++x.st == MLA_SB) x.st = 0, x.phase_b ^= 1;
         return true;
     }
     __device__ void issue() {
-        Issue x{uni(c->tmem), uni(umma_smem_u32(ring_b)), uni(umma_smem_u32(ring_a)), uni(umma_smem_u32(sq)), 0, 0, 0, 0, 0};
+        Issue x{uni(c->tmem), uni(umma_smem_u32(ring_b)), uni(umma_smem_u32(ring_a)), uni(umma_smem_u32(ring_r)), uni(umma_smem_u32(sq)), 0, 0, 0, 0, 0};
         MlaWalk w = walk();
         MlaSeg g;
         int it = 0, seg = 0, prev = 0;   // tiles, segments so far; the stage of the tile before
@@ -429,7 +502,7 @@ struct MlaKernel {
         bool ok = true;
         while (__all_sync(0xffffffffu, ok && w.next(g, seq_at))) {
             const int n = uni(g.tile1 - g.tile0);
-            ok = tc_wait_warp(&c->q_ready, seg & 1);
+            ok = wait_phase(&c->q_ready, seg & 1);
             seg++;
             for (int t = 0; __all_sync(0xffffffffu, ok && t < n); t++, it++) {
                 const int st = x.st;
@@ -440,9 +513,10 @@ struct MlaKernel {
             if (__all_sync(0xffffffffu, ok)) ok = output(x, it - 1, prev, 0, n > 1);
         }
         if (!ok) give_up();
-        // nothing of this warp's is in flight when the CTA ends
-        umma_commit_warp(&c->drain);
-        tc_wait_warp(&c->drain, 0);
+        // nothing of this warp's is in flight when the CTA ends, nor an arrival of the other CTA's on a barrier here
+        if (FP8) umma_commit_to_warp(&c->drain, 3);
+        else umma_commit_warp(&c->drain);
+        wait_phase(&c->drain, 0);
     }
     static __device__ __forceinline__ uint32_t uni(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
     // tensor-memory column of the query chunk at place p
@@ -455,7 +529,7 @@ struct MlaKernel {
     // The output product of tile i is done.  Each parity has a barrier: this warp has seen the scores of tile i or i + 1,
     // so the product of tile i - 2 is done and the barrier at most one phase behind (a wait by parity that is two phases
     // behind would never end).
-    __device__ __forceinline__ bool output_done(int i) { return tc_wait_warp(&c->pv_done[i & 1], (i >> 1) & 1); }
+    __device__ __forceinline__ bool output_done(int i) { return wait_phase(&c->pv_done[i & 1], (i >> 1) & 1); }
 
     // ---- softmax and output: 4 warps, one query row per thread
     __device__ void rows() {
@@ -464,36 +538,39 @@ struct MlaKernel {
         // scores in units of log2: a negative scale flips the query's signs, a scale of zero makes the query zero, so
         // that the factor is positive and the largest product gives the largest score
         const float c2 = q.scale == 0.0f ? 1.0f : fabsf(q.scale) * 1.4426950408889634f;
-        MlaWalk w = walk();
-        MlaSeg g;
+        MlaCtl::Rows &u = c->rows[warp & 3];
+        const MlaSeg &g = u.g;
+        const MlaSeq &s = u.w.s;
+        if (lane == 0) u.w = walk();
         int it = 0;
         bool ok = true;
-        while (ok && w.next(g, seq_at)) {
-            const MlaSeq s = w.s;
+        for (;;) {
+            if (lane == 0) u.more = ok && u.w.next(u.g, seq_at);
+            __syncwarp();
+            if (!u.more) break;
             const uint32_t row = (uint32_t)g.block * MLA_M + r;
             const bool live = row < (uint32_t)s.n * q.n_heads;
-            const int token = live ? row / (uint32_t)q.n_heads : 0, head = live ? row - (uint32_t)token * q.n_heads : 0;
+            const int token = live ? row / (uint32_t)q.n_heads : 0;
+            const int tile0 = g.tile0, tile1 = g.tile1, ctx = s.ctx;
             load_query(r, s, (uint32_t)g.block * MLA_M);
             float ref = -INFINITY, l = 0.0f;
-            for (int t = g.tile0; t < g.tile1; t++, it++) {
-                const int st = it % MLA_SB;
+            for (int t = tile0; t < tile1; t++, it++) {
                 const int64_t pos0 = (int64_t)t * MLA_N;
-                ok = tc_wait_warp(&c->s_full[it & 1], (it >> 1) & 1);
+                ok = wait_phase(&c->s_full[it & 1], (it >> 1) & 1);
                 if (!ok) break;
                 tmem_fence_after();
                 // a tile that reaches the drafted rows, or lacks a page: hide what the row does not see
-                const uint64_t pages = *reinterpret_cast<const volatile uint64_t *>(c->valid[st]);
+                const uint64_t pages = *reinterpret_cast<const volatile uint64_t *>(c->valid[it & 3]);
                 uint64_t see = ~0ull, nf = 0;
-                const bool part = pos0 + MLA_N > s.ctx || pages != 0x0101010101010101ull;
+                const bool part = pos0 + MLA_N > ctx || pages != 0x0101010101010101ull;
                 if (part) {
                     see = mla_visible(q, s, token, pos0) & pages * 255;
-                    nf = clean(st, it & 1);
+                    nf = clean(it % MLA_SB, it & 1);
                 }
-                // the scores are read twice (largest, weights), half a tile at a time: all 64 and the weights at once
-                // do not fit 128 registers beside the rest
+                // the scores are read twice (largest, weights), half a tile at a time, in loops that stay rolled
                 const uint32_t ts = tmem + MLA_TM_S + (it & 1) * 64;
                 float v[32], top = -INFINITY;
-#pragma unroll
+#pragma unroll 1
                 for (int h = 0; h < 2; h++) {
                     tmem_ld32(ts + 32 * h, v);
                     if (part) hide(v, (uint32_t)(see >> 32 * h), (uint32_t)(nf >> 32 * h));
@@ -507,7 +584,7 @@ struct MlaKernel {
                     top = fmaxf(fmaxf(m0, m1), v[31]);
                 }
                 top *= c2;
-                if (t == g.tile0) ref = top;
+                if (t == tile0) ref = top;
                 else if (__any_sync(0xffffffffu, top > ref + MLA_RAISE)) {
                     // raise the reference: weights stay below 2^8 of it, so fp16 and bf16 hold them
                     const float m = fmaxf(ref, top), f = m == -INFINITY ? 1.0f : ex2(ref - m);
@@ -516,6 +593,7 @@ struct MlaKernel {
                     ok = output_done(it - 1);   // the output holds all tiles before this one
                     if (!ok) break;
                     tmem_fence_after();
+#pragma unroll 1
                     for (int col = 0; col < half_cols; col += 32) {
                         float o[32];
                         uint32_t u[32];
@@ -529,26 +607,24 @@ struct MlaKernel {
                 const float m0 = ref == -INFINITY ? 0.0f : -ref;
                 const uint64_t cc = pair2(c2, c2), mm = pair2(m0, m0);
                 uint64_t sum[2] = {0, 0};
-                uint32_t pk[32];
-#pragma unroll
+#pragma unroll 1
                 for (int h = 1; h >= 0; h--) {
-                    if (h == 0) {   // the second half is still in registers from the first pass
-                        tmem_ld32(ts, v);
-                        if (part) hide(v, (uint32_t)see, (uint32_t)nf);
-                    }
+                    tmem_ld32(ts + 32 * h, v);
+                    if (part) hide(v, (uint32_t)(see >> 32 * h), (uint32_t)(nf >> 32 * h));
+                    uint32_t pk[16];
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
                         float a, b;
                         unpair2(fma2(pair2(v[k], v[k + 1]), cc, mm), a, b);
                         a = ex2(a), b = ex2(b);
                         sum[k >> 1 & 1] = add2(sum[k >> 1 & 1], pair2(a, b));
-                        pk[16 * h + k / 2] = pack2<BF16>(a, b);
+                        pk[k / 2] = pack2<BF16>(a, b);
                     }
+                    tmem_st16(ts + MLA_TM_P + 16 * h, pk);   // over the second half's scores, which no one reads again
                 }
                 float sa, sb;
                 unpair2(add2(sum[0], sum[1]), sa, sb);
                 l += sa + sb;
-                tmem_st32(ts, pk);
                 tmem_wait_st();
                 tmem_fence_before();
                 __syncwarp();
@@ -558,8 +634,9 @@ struct MlaKernel {
             ok = output_done(it - 1);
             if (!ok) break;
             tmem_fence_after();
-            if (g.whole) store_out(tmem, live, (int64_t)s.q0 + token, head, ref, l);
-            else store_piece(tmem, g, w, live, r, ref, l);
+            if (g.whole) store_out(tmem, live, (int64_t)s.q0 + token, row - (uint32_t)token * q.n_heads, ref, l);
+            else store_piece(tmem, tile0 == 0, live, r, ref, l);
+            __syncwarp();
         }
         if (!ok) give_up();
     }
@@ -574,61 +651,59 @@ struct MlaKernel {
     }
 
     // The block's query rows into tensor memory and shared memory (zeros behind the last row).  A warp loads its own 32
-    // rows, 8 lanes per 128-byte line (a lane per row touches 32 lines with every load: 11,000 cycles a block), so a chunk
-    // for tensor memory passes through shared memory once, from lanes across a row to a lane per row.
-    __device__ __forceinline__ void load_query(int r, const MlaSeq &s, uint32_t row0) {
-        const uint32_t rows = (uint32_t)s.n * q.n_heads;   // below 2^31, as n_tokens * n_heads is
-        const uint32_t flip = q.scale < 0.0f ? 0x80008000u : 0u, tmem = c->tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const __half *ql[8], *qr[8];   // this lane's piece of rows lane / 8 + 4 i
-        bool live[8];
-        const int u = lane & 7;
+    // rows, 8 lanes per 128-byte line (a lane per row touches 32 lines with every load: 11,000 cycles a block).  The
+    // chunks for tensor memory pass through the shared ones' place, from lanes across a row to a lane per row.
+    __device__ __forceinline__ void load_query(int r, const MlaSeq s, uint32_t row0) {
+        const uint32_t tmem = c->tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        uint8_t *mine = sq + (r >> 5) * 4096;   // this warp's rows of a chunk
+        query_lines<0, NQ>(mine, s, row0 + (r & ~31));
+        __syncwarp();
+#pragma unroll 1
+        for (int p = 0; p < NQ; p++) {
+            uint32_t v[32];
+            const uint8_t *src = mine + p * MLA_QCHUNK + (lane >> 3) * 1024 + (lane & 7) * 128;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t row = row0 + (r & ~31) + (lane >> 3) + 4 * i;
-            live[i] = row < rows && q.scale != 0.0f;
-            const uint32_t token = live[i] ? row / (uint32_t)q.n_heads : 0, head = live[i] ? row - token * q.n_heads : 0;
-            ql[i] = reinterpret_cast<const __half *>(q.latent) + (int64_t)(s.q0 + token) * q.lt + head * q.lh + u * 8;
-            qr[i] = reinterpret_cast<const __half *>(q.rope) + (int64_t)(s.q0 + token) * q.rt + head * q.rh + u * 8;
-        }
-        constexpr int D = FP8 ? 2 : 3;   // chunks in flight
-        uint4 xs[D][8];
-        auto load = [&](int p, uint4 (&x)[8]) {
-            const int g = chunk_at(p);
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                x[i] = live[i] ? __ldg(reinterpret_cast<const uint4 *>(g < 2 * NV ? ql[i] + g * 64 : qr[i])) : make_uint4(0, 0, 0, 0);
-        };
-#pragma unroll
-        for (int p = 0; p < D; p++) load(p, xs[p]);
-#pragma unroll
-        for (int p = 0; p < NC; p++) {
-            uint4 (&x)[8] = xs[p % D];
-            uint8_t *dst = sq + (p < NQ ? 0 : p - NQ) * MLA_QCHUNK + (r >> 5) * 4096;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int k = (lane >> 3) + 4 * i;   // row of the warp's 32
-                *reinterpret_cast<uint4 *>(dst + (k >> 3) * 1024 + (k & 7) * 128 + (u ^ (k & 7)) * 16) =
-                    make_uint4(x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip);
+            for (int k = 0; k < 8; k++) {
+                const uint4 y = *reinterpret_cast<const uint4 *>(src + (k ^ (lane & 7)) * 16);
+                v[4 * k] = y.x, v[4 * k + 1] = y.y, v[4 * k + 2] = y.z, v[4 * k + 3] = y.w;
             }
-            if (p + D < NC) load(p + D, x);
-            if (p < NQ) {
-                __syncwarp();
-                uint32_t v[32];
-                const uint8_t *src = dst + (lane >> 3) * 1024 + (lane & 7) * 128;
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const uint4 y = *reinterpret_cast<const uint4 *>(src + (k ^ (lane & 7)) * 16);
-                    v[4 * k] = y.x, v[4 * k + 1] = y.y, v[4 * k + 2] = y.z, v[4 * k + 3] = y.w;
-                }
-                tmem_st32(tmem + q_col(p), v);
-                __syncwarp();
-            }
+            tmem_st32(tmem + q_col(p), v);
         }
+        __syncwarp();
+        if constexpr (NQ < NC) query_lines<NQ, NC>(mine, s, row0 + (r & ~31));
         tmem_wait_st();
         fence_async_smem();
         tmem_fence_before();
         __syncwarp();
         if (lane == 0) tc_arrive(&c->q_ready);
+    }
+    // chunks P0 .. P1 - 1 of 32 rows, swizzled, into consecutive chunks: lane = 16 bytes (lane % 8) of rows lane / 8 + 4 i
+    template <int P0, int P1>
+    __device__ __forceinline__ void query_lines(uint8_t *dst, const MlaSeq &s, uint32_t row0) {
+        const uint32_t rows = (uint32_t)s.n * q.n_heads;   // below 2^31, as n_tokens * n_heads is
+        const uint32_t flip = q.scale < 0.0f ? 0x80008000u : 0u;
+        const int u = lane & 7;
+        const uint32_t my_token = (row0 + lane) / (uint32_t)q.n_heads, my_head = row0 + lane - my_token * q.n_heads;
+#pragma unroll(FP8 ? 4 : 8)
+        for (int i = 0; i < 8; i++) {   // all of them in flight where the registers allow
+            const int k = (lane >> 3) + 4 * i;
+            const bool live = row0 + k < rows && q.scale != 0.0f;
+            uint32_t token = __shfl_sync(0xffffffffu, my_token, k), head = __shfl_sync(0xffffffffu, my_head, k);
+            if (!live) token = head = 0;
+            const __half *ql = reinterpret_cast<const __half *>(q.latent) + (int64_t)(s.q0 + token) * q.lt + head * q.lh + u * 8;
+            const __half *qr = reinterpret_cast<const __half *>(q.rope) + (int64_t)(s.q0 + token) * q.rt + head * q.rh + u * 8;
+            uint4 x[P1 - P0];
+#pragma unroll
+            for (int p = P0; p < P1; p++) {
+                const uint4 *src = reinterpret_cast<const uint4 *>(p == 2 * NV ? qr : ql + chunk_at(p) * 64);
+                x[p - P0] = live ? __ldg(src) : make_uint4(0, 0, 0, 0);
+            }
+            uint8_t *at = dst + (k >> 3) * 1024 + (k & 7) * 128 + (u ^ (k & 7)) * 16;
+#pragma unroll
+            for (int p = P0; p < P1; p++)
+                *reinterpret_cast<uint4 *>(at + (p - P0) * MLA_QCHUNK) =
+                    make_uint4(x[p - P0].x ^ flip, x[p - P0].y ^ flip, x[p - P0].z ^ flip, x[p - P0].w ^ flip);
+        }
     }
 
     // Rows of the tile with an infinity or a NaN among this CTA's output columns become zeros there (a weight of
@@ -668,6 +743,7 @@ struct MlaKernel {
         constexpr int half_cols = 64 * NV;
         const float f = l == 0.0f ? 0.0f : 1.0f / l;
         __half *out = reinterpret_cast<__half *>(q.out) + token * q.ot + head * q.oh + half * half_cols;
+#pragma unroll 1
         for (int col = 0; col < half_cols; col += 32) {
             float o[32];
             tmem_ld32(tmem + col, o);
@@ -686,10 +762,11 @@ struct MlaKernel {
             q.lse[token * q.n_heads + head] = l == 0.0f ? -INFINITY : ref * 0.69314718055994531f + logf(l);
     }
 
-    __device__ __forceinline__ void store_piece(uint32_t tmem, const MlaSeg &g, const MlaWalk &w, bool live, int r, float ref, float l) {
+    __device__ __forceinline__ void store_piece(uint32_t tmem, bool begins, bool live, int r, float ref, float l) {
         const int L = 128 * NV, half_cols = 64 * NV;
-        const int slot = 2 * pair + (g.tile0 == 0);
+        const int slot = 2 * pair + begins;
         float *o = ws.o + ((size_t)slot * L + half * half_cols) * MLA_M + r;
+#pragma unroll 1
         for (int col = 0; col < half_cols; col += 32) {
             float v[32];
             tmem_ld32(tmem + col, v);
@@ -706,25 +783,29 @@ struct MlaKernel {
 };
 
 template <bool BF16, bool FP8, int NV>
-__global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
+__global__ void __launch_bounds__(FP8 ? 256 + 32 * MLA_XW : 256, 1)
     k_mla(MoeKvDev kv, MlaSeqAt seq_at, MoeMlaQuery q, const __grid_constant__ CUtensorMap tm, void *ws, int *error) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     using K = MlaKernel<BF16, FP8, NV>;
     const int pairs = gridDim.x / 2;
-    uint8_t *ring_b = base, *ring_a = ring_b + MLA_SB * NV * MLA_CHUNK, *sq = ring_a + MLA_RA * MLA_CHUNK;
+    uint8_t *ring_b = base, *ring_a = ring_b + MLA_SB * NV * MLA_CHUNK;
+    uint8_t *ring_r = ring_a + NV * MLA_CHUNK, *sq = FP8 ? ring_r + 2 * MLA_CHUNK : ring_a + MLA_RA * MLA_CHUNK;
     MlaCtl *c = reinterpret_cast<MlaCtl *>(sq + mla_q_sm(128 * NV) * MLA_QCHUNK);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int PROD = FP8 ? 8 : 1;
+    constexpr int PROD = FP8 ? MLA_XW : 1;   // arrivals that fill a tile of ring B: the expanding warps, or the TMA's one
     if (tid == 0) {
-        for (int i = 0; i < MLA_RA; i++) tc_mbar_init(&c->full_a[i], PROD), tc_mbar_init(&c->empty_a[i], 1);
-        for (int i = 0; i < MLA_SB; i++) tc_mbar_init(&c->full_b[i], PROD), tc_mbar_init(&c->empty_b[i], 1);
+        for (int i = 0; i < MLA_RA; i++) tc_mbar_init(&c->full_a[i], 1), tc_mbar_init(&c->empty_a[i], 1);
+        for (int i = 0; i < 2; i++) tc_mbar_init(&c->full_r[i], 1), tc_mbar_init(&c->empty_r[i], 1);
+        for (int i = 0; i < MLA_SB; i++) tc_mbar_init(&c->full_b[i], PROD), tc_mbar_init(&c->empty_b[i], FP8 ? 2 : 1);
         tc_mbar_init(&c->s_full[0], 1), tc_mbar_init(&c->s_full[1], 1);
         tc_mbar_init(&c->p_full[0], 4), tc_mbar_init(&c->p_full[1], 4);
         tc_mbar_init(&c->pv_done[0], 1), tc_mbar_init(&c->pv_done[1], 1);
-        tc_mbar_init(&c->q_ready, 4), tc_mbar_init(&c->drain, 1);
+        tc_mbar_init(&c->q_ready, 4), tc_mbar_init(&c->drain, FP8 ? 2 : 1);
         c->dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        if (FP8)
+            for (int i = 0; i < NV; i++) tc_expect(&c->full_a[i], MLA_CHUNK);   // the other CTA's first chunks
     }
     if (warp == 2) tmem_alloc(&c->tmem, 512);
     moe_pdl_wait();
@@ -764,9 +845,10 @@ __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
         c->off0 = off, c->seq0 = b;
     }
     tmem_fence_before();
+    if (FP8) cluster_sync_all();   // the other CTA's barriers are ready
     __syncthreads();
     tmem_fence_after();
-    K k{kv, seq_at, q, &tm, mla_ws(ws, 128 * NV, pairs), error, ring_b, ring_a, sq, c, (int)(blockIdx.x & 1), pair, lane, warp};
+    K k{kv, seq_at, q, &tm, mla_ws(ws, 128 * NV, pairs), error, ring_b, ring_a, ring_r, sq, c, (int)(blockIdx.x & 1), pair, lane, warp};
     if (k.half == 0 && warp == 3 && lane == 0) {
         // the unit that this pair begins and another one ends (k_mla_join); every call writes the entry
         MlaWalk w = k.walk();
@@ -780,12 +862,14 @@ __global__ void __launch_bounds__(FP8 ? 512 : 256, 1)
     }
     if (w0 < w1) {
         if (FP8 && warp >= 8) k.produce_expand();
-        else if (!FP8 && warp == 0) k.produce_tma();
+        else if (warp == 0) k.produce_tma();
         else if (warp == 1) k.issue();
+        else if (FP8 && warp == 2) k.forward();
         else if (warp >= 4 && warp < 8) k.rows();
     }
     __syncwarp();
     tmem_fence_before();
+    if (FP8) cluster_sync_all();   // nothing of the other CTA's reaches this one any more
     __syncthreads();
     if (warp == 2) tmem_free(c->tmem, 512);
 }
@@ -902,18 +986,30 @@ __global__ void __launch_bounds__(MJ_THREADS, 2) k_mla_join(MoeKvDev kv, MlaSeqA
     }
 }
 
-size_t mla_smem(int latent) {
+size_t mla_smem(int latent, bool fp8) {
     const int nv = latent / 128;
-    return 1024 + (size_t)(MLA_SB * nv + MLA_RA) * MLA_CHUNK + (size_t)mla_q_sm(latent) * MLA_QCHUNK + sizeof(MlaCtl);
+    return 1024 + (size_t)(MLA_SB * nv + (fp8 ? nv + 2 : MLA_RA)) * MLA_CHUNK + (size_t)mla_q_sm(latent) * MLA_QCHUNK + sizeof(MlaCtl);
 }
 
 template <bool BF16, bool FP8, int NV>
 void launch(const MoeKvDev &kv, const MlaSeqAt &at, const MoeMlaQuery &q, const CUtensorMap &tm, void *ws, int pairs,
             int *error, cudaStream_t s) {
     static size_t done[MOE_MAX_DEVICES];
-    const size_t smem = mla_smem(kv.latent);
+    const size_t smem = mla_smem(kv.latent, FP8);
     moe_smem_limit(k_mla<BF16, FP8, NV>, smem, done);
-    moe_launch_pdl(k_mla<BF16, FP8, NV>, dim3(2 * pairs), dim3(FP8 ? 512 : 256), smem, s, kv, at, q, tm, ws, error);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * pairs);
+    cfg.blockDim = dim3(FP8 ? 256 + 32 * MLA_XW : 256);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {FP8 ? 2u : 1u, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, k_mla<BF16, FP8, NV>, kv, at, q, tm, ws, error);
     moe_launch_pdl(k_mla_join<BF16>, dim3(4 * pairs), dim3(MJ_THREADS), sizeof(float) * pairs * MLA_M, s, kv, at, q, ws, pairs);
 }
 
@@ -939,10 +1035,10 @@ size_t moe_mla_ws_bytes(int latent, int sms) {
 int moe_launch_mla(const MoeKvDev &kv, const MoeKvBatchDev &b, const MoeMlaQuery &q, void *ws, int sms, int *error,
                    cudaStream_t s, uint64_t *launches) {
     const MlaSeqAt at{b, q.n_heads, kv.page_shift};
-    const bool fp8 = kv.format == MOE_KV_FP8_F16 || kv.format == MOE_KV_FP8_BF16;
     CUtensorMap tm{};
-    if (!fp8 && moe_make_map_f16_sw128(&tm, kv.data, kv.latent + MOE_KV_ROPE, (uint64_t)kv.n_pages << kv.page_shift, 64,
-                                       kv.page_shift >= 6 ? MLA_N : 1u << kv.page_shift))
+    // rows as 16-bit units (8-bit formats: the TMA only loads the rotary values, which start at unit latent / 2)
+    if (moe_make_map_f16_sw128(&tm, kv.data, kv.row_bytes / 2, (uint64_t)kv.n_pages << kv.page_shift, 64,
+                               kv.page_shift >= 6 ? MLA_N : 1u << kv.page_shift))
         return -1;
     switch (kv.format) {
         case MOE_KV_F16: by_latent<false, false>(kv, at, q, tm, ws, mla_pairs(sms), error, s); break;
