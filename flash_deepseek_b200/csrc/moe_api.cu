@@ -121,6 +121,8 @@ struct moe_ctx {
     size_t mb_x = 0, mb_meta = 0, mb_y = 0;
     int *ep_done = nullptr;  // [3] block counters of the pack, pre-combine and final kernels
     unsigned long long *d_seq = nullptr;  // peer-exchange steps completed by this rank (device)
+    moe_rope_config rope_cfg{};  // of the last rotary call, and its frequency table
+    MoeRopeDev rope{};
     int sms = 0;             // multiprocessors of the device
     int *hits = nullptr;     // moe_record_expert_hits target, or nullptr
     bool comm_aborted = false;  // a host wait gave up on an NCCL exchange
@@ -1591,13 +1593,18 @@ int moe_sample_device(moe_ctx *c, const float *d_logits, int T, int vocab, float
 // ---- MLA attention over a paged latent cache (checks: moe_kv_host.h) ---------
 size_t moe_kv_row_bytes(int format, int latent) { return kv_host_row_bytes(format, latent); }
 
-static MoeRopeDev rope_dev(const moe_rope_config *r) {
-    MoeRopeDev d{};
-    d.pairs = r->dim / 2;
-    d.half_layout = r->half_layout ? 1 : 0;
-    d.mscale = r->mscale;
-    kv_rope_turns(r, d.turns);
-    return d;
+// The frequency table of a configuration: formed anew when the configuration differs from the last call's (32 powers
+// take longer than a small launch).
+static const MoeRopeDev &rope_dev(moe_ctx *c, const moe_rope_config *r) {
+    if (c->rope.pairs == 0 || memcmp(&c->rope_cfg, r, sizeof(*r))) {
+        c->rope_cfg = *r;
+        c->rope = MoeRopeDev{};
+        c->rope.pairs = r->dim / 2;
+        c->rope.half_layout = r->half_layout ? 1 : 0;
+        c->rope.mscale = r->mscale;
+        kv_rope_turns(r, c->rope.turns);
+    }
+    return c->rope;
 }
 static MoeKvDev kv_dev(const moe_kv_cache *kv) {
     MoeKvDev d{(uint8_t *)kv->data, kv->format, kv->latent, 0, kv->n_pages, (int)kv_host_row_bytes(kv->format, kv->latent)};
@@ -1616,7 +1623,7 @@ int moe_rope_device(moe_ctx *c, const moe_rope_config *rope, const void *x, int 
         return fail(c, MOE_ERR_ARG, "moe_rope_device: %s", bad);
     if (T == 0 || n_heads == 0) return MOE_OK;
     DeviceScope ds(c->device);
-    moe_launch_rope(rope_dev(rope), x, x_type, xt, xh, y, y_type, yt, yh, d_pos, T, n_heads, head_dim, offset,
+    moe_launch_rope(rope_dev(c, rope), x, x_type, xt, xh, y, y_type, yt, yh, d_pos, T, n_heads, head_dim, offset,
                     stream ? (cudaStream_t)stream : c->stream, &c->launches);
     CK(cudaGetLastError());
     return MOE_OK;
@@ -1630,10 +1637,8 @@ int moe_kv_write_device(moe_ctx *c, const moe_kv_cache *kv, const moe_kv_batch *
     if (!bad) bad = kv_bad_write(b, x, type, stride, d_norm_w, eps, rope, d_pos);
     if (bad) return fail(c, MOE_ERR_ARG, "moe_kv_write_device: %s", bad);
     if (b->n_tokens == 0 || b->n_seqs == 0) return MOE_OK;
-    MoeRopeDev d{};
-    if (rope) d = rope_dev(rope);
     DeviceScope ds(c->device);
-    moe_launch_kv_write(kv_dev(kv), batch_dev(b), x, type, stride, d_norm_w, eps, rope ? &d : nullptr, d_pos,
+    moe_launch_kv_write(kv_dev(kv), batch_dev(b), x, type, stride, d_norm_w, eps, rope ? &rope_dev(c, rope) : nullptr, d_pos,
                         c->plan.error, stream ? (cudaStream_t)stream : c->stream, &c->launches);
     CK(cudaGetLastError());
     return MOE_OK;

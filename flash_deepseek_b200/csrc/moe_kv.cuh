@@ -92,6 +92,21 @@ __device__ __forceinline__ void kv_store8(T *p, const float (&v)[8]) {
     }
 }
 
+// the same 8 values as loaded (2 or 1 registers a pair instead of 2): what a
+// thread holds of loads that are under way
+template <typename T> struct KvRaw8 { uint4 q[sizeof(T) / 2]; };
+template <typename T>
+__device__ __forceinline__ void kv_load_raw(const T *p, KvRaw8<T> &r) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); i++) r.q[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+}
+template <typename T>
+__device__ __forceinline__ void kv_unraw(const KvRaw8<T> &r, float (&v)[8]) {
+    const T *t = reinterpret_cast<const T *>(r.q);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = KvType<T>::to_f(t[i]);
+}
+
 // 4 e4m3 codes (a 32-bit word) to fp32; exact
 __device__ __forceinline__ void kv_e4m3x4(uint32_t w, float *v) {
     const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFF), __NV_E4M3);

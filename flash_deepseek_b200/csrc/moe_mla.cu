@@ -860,6 +860,7 @@ __global__ void __launch_bounds__(FP8 ? 256 + 32 * MLA_XW : 256, 1)
             tail = MlaWs::Tail{g.seq, g.block, mla_last_pair(total, pair, pairs, w1, rest), 1};
         k.ws.tail[pair] = tail;
     }
+    moe_pdl_trigger();   // the join may take the SMs as they come free
     if (w0 < w1) {
         if (FP8 && warp >= 8) k.produce_expand();
         else if (warp == 0) k.produce_tma();
