@@ -141,8 +141,7 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope_any(RopeArgs a, MoeRopeDev 
 // contiguous) and one rotary pair.
 // ---------------------------------------------------------------------------
 constexpr int KV_WARPS = 4;
-// rows of a warp in flight: 1 / 2 / 3 / 4 took 43.4 / 39.4 / 39.6 / 39.5 us for 112,000 8-bit rows read, 23.7 / 22.4 / 23.9 /
-// 25.2 us for 32,762 written
+// rows of a reading warp in flight: 1 / 2 / 3 / 4 took 43.4 / 39.4 / 39.6 / 39.5 us for 112,000 8-bit rows
 constexpr int KV_RPW = 2;
 constexpr int KV_CHUNKS = 2;   // 256-value chunks of the widest latent part (512)
 
@@ -150,6 +149,96 @@ __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
+}
+
+// One row per warp: the row's own loads are issued before the page lookup, which waits for three dependent ones.  (Two
+// rows per warp as in the read: 28.8 against 25.0 us for 32,762 fp32 rows into 8 bits; more registers, fewer warps.)
+template <typename TI, typename TC, bool FP8, bool VEC>
+__global__ void __launch_bounds__(KV_WARPS * 32) k_kv_write(MoeKvDev kv, MoeKvBatchDev b, const TI *__restrict__ x,
+                                                            long long stride, const float *__restrict__ norm_w,
+                                                            float eps, int rotate, MoeRopeDev rope,
+                                                            const int *__restrict__ pos, int *error) {
+    const int t = blockIdx.x * KV_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (t >= b.n_tokens) return;
+    const int L = kv.latent;
+    const TI *row = x + (long long)t * stride;
+    // the row itself first: these loads do not wait for the page lookup
+    float v[KV_CHUNKS][8], w[KV_CHUNKS][8];
+#pragma unroll
+    for (int c = 0; c < KV_CHUNKS; c++) {
+        const int e = c * 256 + lane * 8;
+        if (e < L) {
+            kv_load8<TI, VEC>(row + e, v[c]);
+            if (norm_w) kv_load8<float, VEC>(norm_w + e, w[c]);
+        }
+    }
+    const int ia = rotate && rope.half_layout ? lane : 2 * lane;
+    const int ib = rotate && rope.half_layout ? lane + MOE_KV_ROPE / 2 : 2 * lane + 1;
+    float ra = KvType<TI>::to_f(row[L + ia]), rb = KvType<TI>::to_f(row[L + ib]);
+    float cs = 1.0f, sn = 0.0f;
+    if (rotate) kv_cos_sin(__ldg(pos + t), rope.turns[lane], rope.mscale, cs, sn);
+    const int seq = kv_seq_of(b, t);
+    if (seq < 0) return;   // behind the last sequence: nothing is written
+    const long long at = kv_flat_row(kv, b, seq, (long long)__ldg(b.ctx_len + seq) + (t - __ldg(b.q_start + seq)));
+    if (at < 0) {
+        if (lane == 0) kv_error(error, KV_ERR_BATCH);
+        return;
+    }
+    if (norm_w) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int c = 0; c < KV_CHUNKS; c++)
+            if (c * 256 + lane * 8 < L)
+#pragma unroll
+                for (int k = 0; k < 8; k++) ss = fmaf(v[c][k], v[c][k], ss);
+        const float r = 1.0f / sqrtf(warp_sum(ss) / (float)L + eps);
+#pragma unroll
+        for (int c = 0; c < KV_CHUNKS; c++)
+            if (c * 256 + lane * 8 < L)
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[c][k] = v[c][k] * r * w[c][k];
+    }
+    if (rotate) {
+        const float a = ra;
+        ra = a * cs - rb * sn;
+        rb = a * sn + rb * cs;
+    }
+    uint8_t *dst = kv.data + at * kv.row_bytes;
+    TC *drope = reinterpret_cast<TC *>(dst + (FP8 ? L : 2 * L));
+#pragma unroll
+    for (int c = 0; c < KV_CHUNKS; c++) {
+        const int e = c * 256 + lane * 8;
+        if (!FP8) {
+            if (e < L) kv_store8<TC, true>(reinterpret_cast<TC *>(dst) + e, v[c]);
+            continue;
+        }
+        // the group's largest magnitude over its 4 lanes (every lane takes
+        // part in the shuffles; L is a multiple of 128, so groups are whole)
+        uint32_t big = 0;
+        if (e < L)
+#pragma unroll
+            for (int k = 0; k < 8; k++) big = max(big, __float_as_uint(v[c][k]) & 0x7FFFFFFFu);
+        big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        if (e >= L) continue;
+        // the least k with amax <= 448 * 2^k, 448 = 1.75 * 2^8 (exact: exponent and mantissa compared as integers)
+        int k = (int)(big >> 23) - 127 - 8 + ((big & 0x7FFFFFu) > 0x600000u);
+        k = min(max(k, KV_K_MIN), KV_K_MAX);
+        const bool bad = big >= 0x7F800000u;
+        const float inv = __uint_as_float((uint32_t)(127 - k) << 23);
+        uint32_t q[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float2 lo = make_float2(v[c][4 * i] * inv, v[c][4 * i + 1] * inv);
+            const float2 hi = make_float2(v[c][4 * i + 2] * inv, v[c][4 * i + 3] * inv);
+            q[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3) |
+                   (uint32_t)__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3) << 16;
+        }
+        *reinterpret_cast<uint2 *>(dst + e) = make_uint2(q[0], q[1]);
+        if ((lane & 3) == 0) dst[L + 2 * MOE_KV_ROPE + e / KV_GROUP] = bad ? 255 : (uint8_t)(127 + k);
+    }
+    drope[ia] = KvType<TC>::from_f(ra);
+    drope[ib] = KvType<TC>::from_f(rb);
 }
 
 // the flat row of row t0 + lane of a warp's RPW rows: -2 in no sequence, -1 (reported) without a page
@@ -162,112 +251,6 @@ __device__ __forceinline__ long long kv_lookup(const MoeKvDev &kv, const MoeKvBa
     const long long at = kv_flat_row(kv, b, seq, (long long)__ldg(b.ctx_len + seq) + (t - __ldg(b.q_start + seq)));
     if (at < 0) kv_error(error, KV_ERR_BATCH);
     return at;
-}
-
-template <typename TI, typename TC, bool FP8, bool VEC, int RPW>
-__global__ void __launch_bounds__(KV_WARPS * 32) k_kv_write(MoeKvDev kv, MoeKvBatchDev b, const TI *__restrict__ x,
-                                                            long long stride, const float *__restrict__ norm_w,
-                                                            float eps, int rotate, MoeRopeDev rope,
-                                                            const int *__restrict__ pos, int *error) {
-    const int t0 = (blockIdx.x * KV_WARPS + (threadIdx.x >> 5)) * RPW, lane = threadIdx.x & 31;
-    if (t0 >= b.n_tokens) return;
-    const int L = kv.latent;
-    const int ia = rotate && rope.half_layout ? lane : 2 * lane;
-    const int ib = rotate && rope.half_layout ? lane + MOE_KV_ROPE / 2 : 2 * lane + 1;
-    // the rows themselves first: these loads do not wait for the page lookup
-    KvRaw8<TI> raw[RPW][KV_CHUNKS];
-    TI ra[RPW], rb[RPW];
-    int ps[RPW];
-#pragma unroll
-    for (int k = 0; k < RPW; k++) {
-        if (t0 + k >= b.n_tokens) break;
-        const TI *row = x + (long long)(t0 + k) * stride;
-#pragma unroll
-        for (int c = 0; c < KV_CHUNKS; c++) {
-            const int e = c * 256 + lane * 8;
-            if (e >= L) continue;
-            if (VEC) kv_load_raw<TI>(row + e, raw[k][c]);
-            else
-#pragma unroll
-                for (int j = 0; j < 8; j++) reinterpret_cast<TI *>(raw[k][c].q)[j] = row[e + j];
-        }
-        ra[k] = row[L + ia];
-        rb[k] = row[L + ib];
-        ps[k] = rotate ? __ldg(pos + t0 + k) : 0;
-    }
-    const long long found = kv_lookup<RPW>(kv, b, t0, lane, error);
-#pragma unroll
-    for (int k = 0; k < RPW; k++) {
-        const long long at = __shfl_sync(0xffffffffu, found, k);
-        if (at < 0) continue;   // no page, or behind the last sequence: nothing is written
-        float v[KV_CHUNKS][8];
-        float ss = 0.0f;
-#pragma unroll
-        for (int c = 0; c < KV_CHUNKS; c++)
-            if (c * 256 + lane * 8 < L) {
-                kv_unraw<TI>(raw[k][c], v[c]);
-#pragma unroll
-                for (int j = 0; j < 8; j++) ss = fmaf(v[c][j], v[c][j], ss);
-            }
-        if (norm_w) {
-            const float r = 1.0f / sqrtf(warp_sum(ss) / (float)L + eps);
-#pragma unroll
-            for (int c = 0; c < KV_CHUNKS; c++)
-                if (c * 256 + lane * 8 < L) {
-                    float w[8];
-                    kv_load8<float, VEC>(norm_w + c * 256 + lane * 8, w);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[c][j] = v[c][j] * r * w[j];
-                }
-        }
-        float u0 = KvType<TI>::to_f(ra[k]), u1 = KvType<TI>::to_f(rb[k]);
-        if (rotate) {
-            float cs, sn;
-            kv_cos_sin(ps[k], rope.turns[lane], rope.mscale, cs, sn);
-            const float a = u0;
-            u0 = a * cs - u1 * sn;
-            u1 = a * sn + u1 * cs;
-        }
-        uint8_t *dst = kv.data + at * kv.row_bytes;
-        TC *drope = reinterpret_cast<TC *>(dst + (FP8 ? L : 2 * L));
-#pragma unroll
-        for (int c = 0; c < KV_CHUNKS; c++) {
-            const int e = c * 256 + lane * 8;
-            if (!FP8) {
-                if (e < L) kv_store8<TC, true>(reinterpret_cast<TC *>(dst) + e, v[c]);
-                continue;
-            }
-            // the group's largest magnitude over its 4 lanes (every lane takes
-            // part in the shuffles; L is a multiple of 128, so groups are whole)
-            uint32_t big = 0;
-            if (e < L)
-#pragma unroll
-                for (int j = 0; j < 8; j++) big = max(big, __float_as_uint(v[c][j]) & 0x7FFFFFFFu);
-            big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-            big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-            if (e < L) {
-                // the least exponent with amax <= 448 * 2^exponent, 448 = 1.75 * 2^8 (exact: exponent and mantissa
-                // compared as integers)
-                int ex = (int)(big >> 23) - 127 - 8 + ((big & 0x7FFFFFu) > 0x600000u);
-                ex = min(max(ex, KV_K_MIN), KV_K_MAX);
-                const bool bad = big >= 0x7F800000u;
-                const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
-                uint32_t q[2];
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const float2 lo = make_float2(v[c][4 * i] * inv, v[c][4 * i + 1] * inv);
-                    const float2 hi = make_float2(v[c][4 * i + 2] * inv, v[c][4 * i + 3] * inv);
-                    q[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3) |
-                           (uint32_t)__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3) << 16;
-                }
-                *reinterpret_cast<uint2 *>(dst + e) = make_uint2(q[0], q[1]);
-                if ((lane & 3) == 0) dst[L + 2 * MOE_KV_ROPE + e / KV_GROUP] = bad ? 255 : (uint8_t)(127 + ex);
-            }
-            __syncwarp();
-        }
-        drope[ia] = KvType<TC>::from_f(u0);
-        drope[ib] = KvType<TC>::from_f(u1);
-    }
 }
 
 // A warp reads RPW rows, all of their loads in front of the first store; lane k looks up row k.
@@ -386,7 +369,7 @@ void moe_launch_kv_write(const MoeKvDev &kv, const MoeKvBatchDev &b, const void 
                          cudaStream_t s, uint64_t *launches) {
     if (b.n_tokens <= 0 || b.n_seqs <= 0) return;
     const bool vec = aligned16(x, stride * type_size(type)) && ((uintptr_t)norm_w & 15) == 0;
-    const int rpw = rows_per_warp(b.n_tokens), grid = (b.n_tokens + KV_WARPS * rpw - 1) / (KV_WARPS * rpw);
+    const int grid = (b.n_tokens + KV_WARPS - 1) / KV_WARPS;
     MoeRopeDev none{};
     const MoeRopeDev &r = rope ? *rope : none;
     const int rotate = rope ? 1 : 0;
@@ -396,9 +379,8 @@ void moe_launch_kv_write(const MoeKvDev &kv, const MoeKvBatchDev &b, const void 
             using TC = decltype(tc);
             constexpr bool F = decltype(fp8)::value;
             const TI *p = reinterpret_cast<const TI *>(x);
-            auto kernel = rpw == 1 ? (vec ? k_kv_write<TI, TC, F, true, 1> : k_kv_write<TI, TC, F, false, 1>)
-                                   : (vec ? k_kv_write<TI, TC, F, true, KV_RPW> : k_kv_write<TI, TC, F, false, KV_RPW>);
-            kernel<<<grid, KV_WARPS * 32, 0, s>>>(kv, b, p, stride, norm_w, eps, rotate, r, pos, error);
+            if (vec) k_kv_write<TI, TC, F, true><<<grid, KV_WARPS * 32, 0, s>>>(kv, b, p, stride, norm_w, eps, rotate, r, pos, error);
+            else k_kv_write<TI, TC, F, false><<<grid, KV_WARPS * 32, 0, s>>>(kv, b, p, stride, norm_w, eps, rotate, r, pos, error);
         });
     });
     LAUNCH_COUNT(launches);
