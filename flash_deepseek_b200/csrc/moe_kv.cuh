@@ -98,7 +98,7 @@ template <typename T> struct KvRaw8 { uint4 q[sizeof(T) / 2]; };
 template <typename T>
 __device__ __forceinline__ void kv_load_raw(const T *p, KvRaw8<T> &r) {
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) / 2); i++) r.q[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    for (int i = 0; i < (int)(sizeof(T) / 2); i++) r.q[i] = reinterpret_cast<const uint4 *>(p)[i];   // (in place: not read-only)
 }
 template <typename T>
 __device__ __forceinline__ void kv_unraw(const KvRaw8<T> &r, float (&v)[8]) {

@@ -38,7 +38,7 @@ inline const char *kv_bad_cache(const moe_kv_cache *kv, const moe_kv_batch *b) {
         return "page_size is not a power of two in 8..1024";
     if (kv->n_pages <= 0 || (int64_t)kv->n_pages * kv->page_size > 0x7FFFFFFFll) return "n_pages out of range";
     if (!kv->data || kv_off(kv->data, 128)) return "cache buffer null or not 128-byte aligned";
-    if (b->n_seqs < 0 || b->n_seqs > 4096 || b->n_tokens < 0) return "number of sequences or tokens out of range";
+    if (b->n_seqs < 0 || b->n_seqs > 4096 || b->n_tokens < 0 || b->n_tokens > (1 << 30)) return "number of sequences or tokens out of range";
     if (b->n_seqs > 0 && (!b->q_start || !b->ctx_len || !b->pages || b->pages_per_seq <= 0 || kv_off(b->q_start, 4) ||
                           kv_off(b->ctx_len, 4) || kv_off(b->pages, 4)))
         return "sequence bounds or page table null or not aligned";
@@ -79,7 +79,7 @@ inline const char *kv_bad_rope_call(const moe_rope_config *rope, const void *x, 
                                     int n_heads, int head_dim, int offset) {
     if (const char *bad = kv_bad_rope(rope)) return bad;
     if (!kv_float_type(x_type) || !kv_float_type(y_type)) return "type not supported";
-    if (T < 0 || n_heads < 0 || n_heads > 65536 || head_dim <= 0 || head_dim > 65536 || offset < 0 ||
+    if (T < 0 || T > (1 << 30) || n_heads < 0 || n_heads > 65536 || head_dim <= 0 || head_dim > 65536 || offset < 0 ||
         offset > head_dim - rope->dim || (int64_t)n_heads * head_dim > 0x3FFFFFFF)
         return "tokens, heads or rotated values out of range";
     if (xt < 0 || xh < 0 || yt < 0 || yh < 0) return "negative stride";

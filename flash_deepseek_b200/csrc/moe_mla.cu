@@ -46,9 +46,7 @@ constexpr int MLA_SB = 3;                   // tiles of ring B
 // Tensor-memory columns: the output from 0 (at most 256), two score tiles of 64 (the weights of a tile, 32 columns of
 // 16-bit pairs, take the place of its second half), the query's chunks.
 constexpr int MLA_TM_S = 256, MLA_TM_P = 32, MLA_TM_Q = 384;
-#ifndef MLA_XW
-#define MLA_XW 8                            // warps that expand the 8-bit formats (8 or 4)
-#endif
+constexpr int MLA_XW = 8;                   // warps that expand the 8-bit formats (4: 667 us where 8 take 626)
 constexpr float MLA_RAISE = 8.0f;           // log2: how far scores may pass the reference before it is raised
 
 // Tensor memory left for query chunks of 32 columns (64 values) each: all of
@@ -80,6 +78,7 @@ struct MlaCtl {   // control block behind the tiles
     int64_t total;
     int seq0;
     uint32_t tmem;
+    int used;                    // 8-bit formats: tiles whose copies the other CTA's scores are done with
     int dead;                    // a bounded wait gave up
 };
 
@@ -391,14 +390,19 @@ struct MlaKernel {
     __device__ void forward() {
         const int n = (int)(c->w1 - c->w0);
         const uint32_t other = half ^ 1, ra = cluster_map(ring_a, other), fa = cluster_map(c->full_a, other);
-        for (int i = 0; i < n; i++) {
+        for (int i = 0; i <= n; i++) {
             const int st = i % MLA_SB;
-            if (!wait_phase(&c->full_b[st], (i / MLA_SB) & 1)) return stop_forward();
-            for (int p = 0; p < NV; p++) {
+            if (i < n && !wait_phase(&c->full_b[st], (i / MLA_SB) & 1)) return stop_forward();
+#pragma unroll 1
+            for (int p = 0; p < NV; p++) {   // the slot: its tile i - 1 is used
                 if (!wait_phase(&c->empty_a[p], (i + 1) & 1)) return stop_forward();
-                if (lane == 0) cluster_copy_async(ra + p * MLA_CHUNK, ring_b + (st * NV + p) * MLA_CHUNK, MLA_CHUNK, fa + p * 8);
+                if (lane == 0 && i < n)
+                    cluster_copy_async(ra + p * MLA_CHUNK, ring_b + (st * NV + p) * MLA_CHUNK, MLA_CHUNK, fa + p * 8);
             }
-            if (i > 0 && lane == 0) tc_arrive(&c->empty_b[(i - 1) % MLA_SB]);
+            if (lane == 0 && i > 0) {
+                *reinterpret_cast<volatile int *>(&c->used) = i;
+                tc_arrive(&c->empty_b[(i - 1) % MLA_SB]);
+            }
             __syncwarp();
         }
     }
@@ -565,6 +569,8 @@ struct MlaKernel {
                 const bool part = pos0 + MLA_N > ctx || pages != 0x0101010101010101ull;
                 if (part) {
                     see = mla_visible(q, s, token, pos0) & pages * 255;
+                    ok = !FP8 || copies_used(it);
+                    if (!ok) break;
                     nf = clean(it % MLA_SB, it & 1);
                 }
                 // the scores are read twice (largest, weights), half a tile at a time, in loops that stay rolled
@@ -706,6 +712,13 @@ struct MlaKernel {
         }
     }
 
+    // Before rows of a tile are changed here (clean), the other CTA has to be done with what is copied from them.
+    __device__ __forceinline__ bool copies_used(int it) {
+        const long long t0 = clock64();
+        bool ok = true;
+        while (ok && *reinterpret_cast<volatile int *>(&c->used) <= it) ok = clock64() - t0 <= TC_WAIT_CYCLES;
+        return __all_sync(0xffffffffu, ok);
+    }
     // Rows of the tile with an infinity or a NaN among this CTA's output columns become zeros there (a weight of
     // zero times a NaN is a NaN), and are named to the caller.  Two threads per row.
     __device__ __forceinline__ uint64_t clean(int st, int par) {
@@ -802,7 +815,7 @@ __global__ void __launch_bounds__(FP8 ? 256 + 32 * MLA_XW : 256, 1)
         tc_mbar_init(&c->p_full[0], 4), tc_mbar_init(&c->p_full[1], 4);
         tc_mbar_init(&c->pv_done[0], 1), tc_mbar_init(&c->pv_done[1], 1);
         tc_mbar_init(&c->q_ready, 4), tc_mbar_init(&c->drain, FP8 ? 2 : 1);
-        c->dead = 0;
+        c->dead = 0, c->used = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         if (FP8)
             for (int i = 0; i < NV; i++) tc_expect(&c->full_a[i], MLA_CHUNK);   // the other CTA's first chunks

@@ -25,7 +25,7 @@ int main() {
     KV("format", format, 2) KV("latent_odd", latent, 500) KV("latent_big", latent, 640) KV("latent_0", latent, 0)
     KV("page_48", page_size, 48) KV("page_4", page_size, 4) KV("page_2048", page_size, 2048) KV("page_neg", page_size, -64)
     KV("pages_0", n_pages, 0) KV("pages_many", n_pages, 1 << 26) KV("data_null", data, nullptr) KV("data_off", data, mem + 16)
-    BT("seqs_neg", n_seqs, -1) BT("seqs_many", n_seqs, 4097) BT("tokens_neg", n_tokens, -1) BT("start_null", q_start, nullptr)
+    BT("seqs_neg", n_seqs, -1) BT("seqs_many", n_seqs, 4097) BT("tokens_neg", n_tokens, -1) BT("tokens_many", n_tokens, (1 << 30) + 1) BT("start_null", q_start, nullptr)
     BT("ctx_null", ctx_len, nullptr) BT("table_null", pages, nullptr) BT("table_0", pages_per_seq, 0)
     { moe_kv_batch k{0, 0, nullptr, nullptr, nullptr, 0}; say("no_seqs", kv_bad_cache(&kv, &k)); }
 
@@ -45,6 +45,7 @@ int main() {
     rope("rope_neg", r, mem, 1, -192, 64, y, 1, 192, 64, 2, 3, 64, 0);
     rope("rope_off_align", r, mem + 1, 1, 192, 64, y, 1, 192, 64, 2, 3, 64, 0);
     rope("rope_nothing", r, nullptr, 1, 192, 64, nullptr, 1, 192, 64, 0, 3, 64, 0);
+    rope("rope_many", r, mem, 1, 192, 64, y, 1, 192, 64, (1 << 30) + 1, 3, 64, 0);
     rope("rope_null", r, nullptr, 1, 192, 64, y, 1, 192, 64, 1, 3, 64, 0);
     rope("rope_broadcast_in", r, mem, 1, 0, 0, y, 1, 192, 64, 2, 3, 64, 0);
 #define RP(name, field, value) { moe_rope_config k = r; k.field = value; say(name, kv_bad_rope(&k)); }

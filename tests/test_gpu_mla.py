@@ -451,6 +451,74 @@ def test_attend_masks_that_leave_rows_empty_and_nan_rows(m, cuda_lib, fmt, ctx):
         assert np.all(out[0] == 0) and np.all(np.isneginf(lse[0]))
 
 
+@pytest.mark.parametrize("fmt", R.FORMATS)
+@pytest.mark.parametrize("column", [5, 300, 540])
+def test_attend_one_nan_spoils_the_whole_row_that_sees_it(m, cuda_lib, fmt, column):
+    """A NaN in one half of a drafted row's latent values, or in its rotary ones, reaches every output of the tokens
+    that see it, in both halves, call after call; the others are as without it."""
+    lens = [(3 + 70 * k, 4) for k in range(40)]
+    g = Paged(cuda_lib, lens, fmt, 512, 64, seed=5)
+    fill(g, 5)
+    sees = np.tril(np.ones((4, 4), bool))
+    sees[3, 2] = False
+    for b, (c, n) in enumerate(lens):
+        row = g.host[g.rows(b, c + 2, c + 3)].copy()
+        if R.is_fp8(fmt) and column < 512:
+            row[0, 640 + column // 32] = 255
+        else:
+            at = column if not R.is_fp8(fmt) else 256 + column - 512
+            row.view(np.uint16)[0, at] = 0x7FFF
+        g.host[g.rows(b, c + 2, c + 3)] = row
+    g.upload()
+    q = np.random.default_rng(4).standard_normal((g.T, 16, 576))
+    tree = np.tile(pack_tree(sees, 1), (len(lens), 1))
+    t = R.kind(fmt)
+    for _ in range(5):
+        out, lse = run_attend(m, g, q, 0.1, t, tree=tree)
+        for b, (c, n) in enumerate(lens):
+            o = out[g.start[b]:g.start[b + 1]]
+            assert np.all(np.isnan(o[2])) and not np.any(np.isnan(o[[0, 1, 3]])), b
+    keep = [0, 1, 3]
+    for b in (0, 1, 39):
+        c, n = lens[b]
+        kv = R.unpack(g.host[g.rows(b, 0, c + n)], 512, fmt)
+        vis = np.concatenate([np.ones((n, c), bool), sees], 1)[keep]
+        sl = slice(g.start[b], g.start[b + 1])
+        want, wl, A, S = R.attend(R.rounded(q[sl], t)[keep], kv, vis, 0.1, 512)
+        tol, tl = R.attend_bounds(want, wl, A, S, t)
+        assert np.all(np.abs(out[sl][keep] - want) <= tol) and np.all(np.abs(lse[sl][keep] - wl) <= tl)
+
+
+def test_bounds_out_of_range_skip_the_sequence(m, cuda_lib):
+    """A sequence whose rows pass the call's, or whose context is negative, is skipped by the attention; one whose
+    context passes its page table sees what the table holds; both are reported, the others are right."""
+    F = cuda_lib
+    lens = [(40, 2), (70, 3), (9, 2)]
+    g = Paged(F, lens, R.FP8_BF16, 256, 16, seed=2)
+    fill(g, 2)
+    q = np.random.default_rng(3).standard_normal((7, 20, 320))
+    chain = [np.tril(np.ones((n, n), bool)) for _, n in lens]
+    for starts, ctx in (([0, 2, 5, 9], [40, 70, 9]), ([0, 2, 5, 7], [40, 70, -1])):
+        g.bufs[0], g.bufs[1] = dev(np.array(starts, np.int32)), dev(np.array(ctx, np.int32))
+        out, lse = run_attend(m, g, q, 0.2, "bf16", check=False)
+        with pytest.raises(F.MoeError, match="bounds"):
+            m.check_error()
+        two = [(40, 2), (70, 3)]
+        g.lens, keep = two, g.lens
+        check_attend(g, q, 0.2, out, lse, chain[:2])
+        g.lens = keep
+        assert np.all(out[5:] == 7) and np.all(lse[5:] == 7)
+    # a context past the table (5 pages of 16 rows): the 80 rows that the table holds, of which 73 to 79 were never
+    # written and hold NaN patterns, so every weighted sum over them is NaN
+    g.bufs[0], g.bufs[1] = dev(g.start), dev(np.array([40, 10 ** 6, 9], np.int32))
+    out, lse = run_attend(m, g, q, 0.2, "bf16", check=False)
+    with pytest.raises(F.MoeError, match="bounds"):
+        m.check_error()
+    assert np.all(np.isnan(out[2:5])) and np.all(np.isfinite(out[5:]))
+    g.lens = [(40, 2)]
+    check_attend(g, q, 0.2, out, lse, chain[:1])
+
+
 @pytest.mark.parametrize("fmt", [R.F16, R.FP8_BF16])
 def test_attend_strides(m, cuda_lib, fmt):
     """Padded rows; heads in front of tokens; no lse."""
