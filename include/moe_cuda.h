@@ -245,10 +245,11 @@ uint32_t moe_rng_advance(uint32_t state, int n);
  * they can be captured into CUDA graphs, and calls on different streams may
  * overlap as long as they do not write the same buffers (moe_mla_attention:
  * the same workspace).  Arguments that live on the device (sequence bounds,
- * page tables) are checked by the kernels: a token whose row lies outside its
- * page table, or whose page is out of range, is skipped (moe_kv_write), reads
- * as zeros (moe_kv_read) or is treated as a row that nobody sees
- * (moe_mla_attention), and moe_check_error() reports MOE_ERR_ARG. */
+ * page tables) are checked by the kernels: a row that lies outside its page
+ * table, or whose page is out of range, is skipped (moe_kv_write), reads as
+ * zeros (moe_kv_read) or is seen by nobody (moe_mla_attention, which also skips
+ * a sequence whose bounds pass the call's rows or whose context is negative),
+ * and moe_check_error() reports MOE_ERR_ARG. */
 #define MOE_KV_ROPE 64      /* rotary values of a cache row (QK_ROPE_HEAD_DIM) */
 #define MOE_KV_F16 1        /* rows of (latent + 64) fp16 */
 #define MOE_KV_BF16 30      /* rows of (latent + 64) bf16 */
@@ -275,7 +276,7 @@ typedef struct moe_kv_cache {
  * sequence and are left as they are. */
 typedef struct moe_kv_batch {
     int n_seqs;          /* 0 .. 4096 */
-    int n_tokens;        /* rows of the call's buffers */
+    int n_tokens;        /* rows of the call's buffers, 0 .. 2^30 */
     const int *q_start;  /* device [n_seqs + 1], ascending */
     const int *ctx_len;  /* device [n_seqs] */
     const int *pages;    /* device [n_seqs][pages_per_seq] */
@@ -337,8 +338,10 @@ int moe_kv_read_device(moe_ctx *ctx, const moe_kv_cache *kv, const moe_kv_batch 
  * d_tree[token][j / 32] for the j-th row of its sequence in this call, itself
  * included.  d_tree NULL: a causal chain (j <= its own number).  Rows that a
  * token does not see never touch its output, whatever they hold; a visible
- * row with an infinity or a NaN makes it NaN.  A token that sees nothing gets
- * out = 0 and lse = -infinity.
+ * row with a NaN makes it NaN (with an infinity: NaN or what IEEE arithmetic
+ * leaves).  A token that sees nothing gets
+ * out = 0 and lse = -infinity.  Rows of the call that tree_words does not
+ * reach are not seen.
  * q_latent [token][head][latent], q_rope [token][head][64], out
  * [token][head][latent] in the cache's 16-bit type (fp16 for MOE_KV_F16 and
  * MOE_KV_FP8_F16, else bf16), strides in elements (multiples of 8), buffers
