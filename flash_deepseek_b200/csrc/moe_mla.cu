@@ -451,9 +451,11 @@ struct MlaKernel {
         constexpr uint32_t id = umma_idesc_16(MLA_M, MLA_N, BF16, 0);
         if (!then_wait(x.seen_b, &c->full_b[x.st], x.phase_b)) return false;
         x.seen_b = 0;   // of this tile only: the first tile of a segment has no output() behind it that tests the next
+        // The score tile it & 1 is free once the product that reads its weights (tile it - 2) is done.  The issue order
+        // does not say so: products of another accumulator and shape are not ordered with it.  (The barrier is at most
+        // one phase behind: the product of tile it itself is issued later.)
+        if (!wait_phase(&c->pv_done[it & 1], ((it >> 1) + 1) & 1)) return false;
         tmem_fence_after();
-        // The score tile it & 1 is free: its weights' product (tile it - 2) was issued before, and the tensor pipe
-        // runs in order
         const uint32_t ts = x.tmem + MLA_TM_S + (it & 1) * 64;
         uint32_t seen_a = 0;
         auto chunk_tm = [&](uint32_t q_at, uint32_t k_at, uint32_t first) {   // the query's chunk in tensor memory
