@@ -135,6 +135,16 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
+// a number handed from one thread of the CTA to others, with what the writer saw and wrote before it
+__device__ __forceinline__ void store_release(int *p, int v) {
+    asm volatile("st.release.cta.shared::cta.s32 [%0], %1;\n" ::"r"(umma_smem_u32(p)), "r"(v) : "memory");
+}
+__device__ __forceinline__ int load_acquire(const int *p) {
+    int v;
+    asm volatile("ld.acquire.cta.shared::cta.s32 %0, [%1];\n" : "=r"(v) : "r"(umma_smem_u32(p)) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -406,7 +416,7 @@ struct MlaKernel {
                     cluster_copy_async(ra + p * MLA_CHUNK, ring_b + (st * NV + p) * MLA_CHUNK, MLA_CHUNK, fa + p * 8);
             }
             if (lane == 0 && i > 0) {
-                *reinterpret_cast<volatile int *>(&c->used) = i;
+                store_release(&c->used, i);
                 tc_arrive(&c->empty_b[(i - 1) % MLA_SB]);
             }
             __syncwarp();
@@ -724,7 +734,7 @@ struct MlaKernel {
     __device__ __forceinline__ bool copies_used(int it) {
         const long long t0 = clock64();
         bool ok = true;
-        while (ok && *reinterpret_cast<volatile int *>(&c->used) <= it) ok = clock64() - t0 <= TC_WAIT_CYCLES;
+        while (ok && load_acquire(&c->used) <= it) ok = clock64() - t0 <= TC_WAIT_CYCLES;
         return __all_sync(0xffffffffu, ok);
     }
     // Rows of the tile with an infinity or a NaN among this CTA's output columns become zeros there (a weight of

@@ -101,3 +101,14 @@ def test_scores_wait_for_the_product_that_reads_their_place(tiles):
 def test_issue_order_alone_orders_no_products_of_different_accumulators():
     bad = unordered(5, {"full_b"})
     assert bad and all(a[0] == "output" and b == ("scores", a[1] + 2) for a, b in bad)
+
+
+def test_numbers_between_warps_are_released_and_acquired():
+    """`used` goes from the copying warp to the softmax warps outside any barrier: a plain store and load of it would
+    order nothing else (the rows that are then overwritten)."""
+    text = open(SRC).read()
+    uses = [m.start() for m in re.finditer(r"c->used\b", text)]
+    handed = [m.end() - len("c->used") for m in re.finditer(r"(?:store_release|load_acquire)\(&c->used", text)]
+    first = text.index("c->used = 0")   # the start value, in front of the block's barrier
+    assert len(handed) == 2 and sorted(handed + [first]) == uses
+    assert "store_release" in body("forward") and "load_acquire" in body("copies_used")
