@@ -73,11 +73,12 @@ struct MlaCtl {   // control block behind the tiles
     uint64_t full_a[MLA_RA], empty_a[MLA_RA], full_b[MLA_SB], empty_b[MLA_SB];   // chunks of ring A, tiles of ring B
     uint64_t full_r[2], empty_r[2];   // 8-bit formats: rotary chunks by tile parity
     uint64_t s_full[2], p_full[2], pv_done[2], q_ready, drain;   // by tile parity
+    uint64_t clean;              // the softmax warps meet (clean)
     uint64_t nonfinite[2];       // by tile parity: rows of a tile with an infinity or a NaN in this CTA's latent half
     struct Rows {                // each softmax warp's walk over the segments (in registers it would cost them 30)
         MlaWalk w;
         MlaSeg g;
-        int more;
+        int more, met;           // met: phases of `clean` so far
     } rows[4];
     uint8_t valid[4][8];         // by tile: 8-row groups whose page exists
     int64_t w0, w1, off0;        // the pair's share: first and last tile, place of the first in its sequence
@@ -563,7 +564,7 @@ struct MlaKernel {
         MlaCtl::Rows &u = c->rows[warp & 3];
         const MlaSeg &g = u.g;
         const MlaSeq &s = u.w.s;
-        if (lane == 0) u.w = walk();
+        if (lane == 0) u.w = walk(), u.met = 0;
         int it = 0;
         bool ok = true;
         for (;;) {
@@ -587,9 +588,8 @@ struct MlaKernel {
                 const bool part = pos0 + MLA_N > ctx || pages != 0x0101010101010101ull;
                 if (part) {
                     see = mla_visible(q, s, token, pos0) & pages * 255;
-                    ok = !FP8 || copies_used(it);
+                    ok = (!FP8 || copies_used(it)) && clean(it % MLA_SB, it & 1, u, nf);
                     if (!ok) break;
-                    nf = clean(it % MLA_SB, it & 1);
                 }
                 // the scores are read twice (largest, weights), half a tile at a time, in loops that stay rolled
                 const uint32_t ts = tmem + MLA_TM_S + (it & 1) * 64;
@@ -737,13 +737,20 @@ struct MlaKernel {
         while (ok && load_acquire(&c->used) <= it) ok = clock64() - t0 <= TC_WAIT_CYCLES;
         return __all_sync(0xffffffffu, ok);
     }
+    // The four softmax warps meet.  By an mbarrier, whose wait is bounded: a warp whose own wait gave up does not come,
+    // and the others must not stand at a block barrier for good.
+    __device__ __forceinline__ bool meet(MlaCtl::Rows &u) {
+        const uint32_t phase = u.met & 1;
+        __syncwarp();
+        if (lane == 0) u.met++, tc_arrive(&c->clean);
+        return wait_phase(&c->clean, phase);
+    }
     // Rows of the tile with an infinity or a NaN among this CTA's output columns become zeros there (a weight of
     // zero times a NaN is a NaN), and are named to the caller.  Two threads per row.
-    __device__ __forceinline__ uint64_t clean(int st, int par) {
+    __device__ __forceinline__ bool clean(int st, int par, MlaCtl::Rows &u, uint64_t &nf) {
         const int tid = (warp & 3) * 32 + lane, r = tid >> 1, h = tid & 1;
         if (tid == 0) c->nonfinite[par] = 0;
-        __syncwarp();
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (!meet(u)) return false;
         const uint32_t top = BF16 ? 0x7F80u : 0x7C00u;
         bool bad = false;
         for (int p = 0; p < NV; p++) {
@@ -751,9 +758,9 @@ struct MlaKernel {
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const uint4 x = src[k];
-                const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+                const uint32_t v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                for (int j = 0; j < 4; j++) bad |= (u[j] & top) == top || (u[j] >> 16 & top) == top;
+                for (int j = 0; j < 4; j++) bad |= (v[j] & top) == top || (v[j] >> 16 & top) == top;
             }
         }
         bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 1) != 0;
@@ -765,9 +772,9 @@ struct MlaKernel {
                     reinterpret_cast<uint4 *>(ring_b + (st * NV + p) * MLA_CHUNK + r * 128 + h * 64)[k] = make_uint4(0, 0, 0, 0);
         }
         fence_async_smem();
-        __syncwarp();
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        return *reinterpret_cast<volatile uint64_t *>(&c->nonfinite[par]);
+        if (!meet(u)) return false;
+        nf = *reinterpret_cast<volatile uint64_t *>(&c->nonfinite[par]);
+        return true;
     }
 
     __device__ __forceinline__ void store_out(uint32_t tmem, bool live, int64_t token, int head, float ref, float l) {
@@ -832,7 +839,7 @@ __global__ void __launch_bounds__(FP8 ? 256 + 32 * MLA_XW : 256, 1)
         tc_mbar_init(&c->s_full[0], 1), tc_mbar_init(&c->s_full[1], 1);
         tc_mbar_init(&c->p_full[0], 4), tc_mbar_init(&c->p_full[1], 4);
         tc_mbar_init(&c->pv_done[0], 1), tc_mbar_init(&c->pv_done[1], 1);
-        tc_mbar_init(&c->q_ready, 4), tc_mbar_init(&c->drain, FP8 ? 2 : 1);
+        tc_mbar_init(&c->q_ready, 4), tc_mbar_init(&c->clean, 4), tc_mbar_init(&c->drain, FP8 ? 2 : 1);
         c->dead = 0, c->used = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         if (FP8)

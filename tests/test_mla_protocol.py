@@ -112,3 +112,63 @@ def test_numbers_between_warps_are_released_and_acquired():
     first = text.index("c->used = 0")   # the start value, in front of the block's barrier
     assert len(handed) == 2 and sorted(handed + [first]) == uses
     assert "store_release" in body("forward") and "load_acquire" in body("copies_used")
+
+
+def test_roles_meet_at_bounded_waits_only():
+    """Every wait of a role gives up after a while and the role returns.  A block barrier among them would hold the
+    other warps for good: only the kernel's entry and exit, which all threads reach, have one."""
+    text = open(SRC).read()
+    roles = text[text.index("struct MlaKernel"):text.index("k_mla(MoeKvDev kv")]
+    assert not re.search(r"bar\.sync|barrier\.sync|__syncthreads|cluster_sync", roles)
+    assert "clean" in body("meet") and body("clean").count("meet(u)") == 2
+
+
+class Phases:
+    """An mbarrier: completed phases, arrivals of the present one."""
+
+    def __init__(self, count):
+        self.count, self.done, self.here = count, 0, 0
+
+    def arrive(self):
+        self.here += 1
+        if self.here == self.count:
+            self.done, self.here = self.done + 1, 0
+
+    def passed(self, parity):
+        return self.done & 1 != parity
+
+
+def softmax_warps(tiles, gives_up, rng, patience=200):
+    """Four warps over tiles that need cleaning, in random order; gives_up: {warp: tile in whose wait it gives up}.
+    Returns for each warp the tiles that it finished; raises if one never returns."""
+    bar, met = Phases(4), [0] * 4
+    done, asleep = [0] * 4, [0] * 4
+    live = {0, 1, 2, 3}
+    arrived = [False] * 4
+    for _ in range(100000):
+        if not live:
+            return done
+        w = rng.choice(sorted(live))
+        if done[w] == tiles or (gives_up.get(w) == done[w] and met[w] == 2 * done[w] and not arrived[w]):
+            live.discard(w)
+        elif not arrived[w]:
+            bar.arrive()
+            arrived[w], asleep[w] = True, 0
+        elif bar.passed(met[w] & 1):
+            met[w], arrived[w] = met[w] + 1, False
+            done[w] = met[w] // 2
+        else:
+            asleep[w] += 1
+            if asleep[w] > patience:
+                live.discard(w)
+    raise AssertionError("a warp never returned")
+
+
+def test_a_warp_that_gives_up_leaves_no_other_behind():
+    import random
+    for seed in range(40):
+        rng = random.Random(seed)
+        assert softmax_warps(6, {}, rng) == [6] * 4
+        w, t = rng.randrange(4), rng.randrange(6)
+        done = softmax_warps(6, {w: t}, rng)
+        assert done[w] == t and all(t <= d <= t + 1 for d in done)
