@@ -27,8 +27,11 @@ struct MlaSeq {
     KV_HD int64_t work() const { return (int64_t)blocks * tiles; }
 };
 
+// (A table may span more rows than an int holds, pages repeated; no sequence gets past 2^31 - 65.)
 KV_HD MlaSeq mla_seq(int q0, int q1, int ctx, int n_tokens, int heads, int64_t table_rows) {
+    constexpr int64_t most = 0x7FFFFFFF - MLA_N;   // s.len and its last tile's end are ints
     MlaSeq s{};
+    if (table_rows > most) table_rows = most;
     if (q0 < 0 || q1 < q0 || q1 > n_tokens || ctx < 0) {
         s.bad = 1;
         return s;

@@ -875,7 +875,7 @@ __global__ void __launch_bounds__(FP8 ? 256 + 32 * MLA_XW : 256, 1)
     if (w0 < w1 && w0 >= before && w0 < before + mine) {
         int64_t off = w0 - before;
         int b = b0;
-        for (;; b++) {
+        for (; b < b1 - 1; b++) {   // w0 lies in this stretch, so in its last sequence if in none before
             const int64_t k = seq_at(b).work();
             if (off < k) break;
             off -= k;
