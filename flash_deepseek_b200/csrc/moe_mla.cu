@@ -89,7 +89,10 @@ struct MlaCtl {   // control block behind the tiles
     int dead;                    // a bounded wait gave up
 };
 
-// Pieces of cut units: [pair][slot][latent][128 rows] sums, [pair][slot][2][128] references and sums of weights
+// Pieces of cut units: [pair][slot][latent][128 rows] sums, [pair][slot][half][2][128] references and sums of weights.
+// Each half of the columns has its CTA's own: the two CTAs sum a score's chunks in different orders, so their scores
+// differ in the last bits, and one may raise its reference where the other does not (by up to MLA_RAISE apart then).
+constexpr int MLA_STATS = 2 * 2 * MLA_M;   // floats of a slot
 struct MlaWs {
     struct Tail {                // the unit that pair p begins and does not end
         int seq, block, last, on;
@@ -103,7 +106,7 @@ __host__ __device__ MlaWs mla_ws(void *ws, int latent, int pairs) {
     w.tail = reinterpret_cast<MlaWs::Tail *>(b);
     b += ((size_t)pairs * sizeof(MlaWs::Tail) + 255) / 256 * 256;
     w.ml = reinterpret_cast<float *>(b);
-    b += (size_t)pairs * 2 * 2 * MLA_M * sizeof(float);
+    b += (size_t)pairs * 2 * MLA_STATS * sizeof(float);
     w.o = reinterpret_cast<float *>(b);
     return w;
 }
@@ -813,9 +816,10 @@ struct MlaKernel {
                 if (live) o[(size_t)(col + k) * MLA_M] = v[k];
             __syncwarp();
         }
-        if (half == 0 && live) {
-            ws.ml[(size_t)slot * 2 * MLA_M + r] = ref;
-            ws.ml[(size_t)slot * 2 * MLA_M + MLA_M + r] = l;
+        if (live) {
+            float *ml = ws.ml + (size_t)slot * MLA_STATS + half * 2 * MLA_M + r;
+            ml[0] = ref;
+            ml[MLA_M] = l;
         }
     }
 };
@@ -969,6 +973,7 @@ __global__ void __launch_bounds__(MJ_THREADS, 2) k_mla_join(MoeKvDev kv, MlaSeqA
     const int per = L / cols, items = n * per;
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
         const int p = units[item / per], col0 = (item % per) * cols;
+        const float *ml = ws.ml + (2 * col0 < L ? 0 : 2 * MLA_M) + r;   // (an item's columns lie in one half)
         const MlaWs::Tail t = ws.tail[p];
         const MlaSeq s = seq_at(t.seq);
         const uint32_t row = (uint32_t)t.block * MLA_M + r;
@@ -978,7 +983,7 @@ __global__ void __launch_bounds__(MJ_THREADS, 2) k_mla_join(MoeKvDev kv, MlaSeqA
         auto slot = [&](int k) { return (size_t)(k == 0 ? 2 * p + 1 : 2 * (p + k)); };
         __syncthreads();
 #pragma unroll 8
-        for (int k = part; k < pieces; k += 4) sw[k * MLA_M + r] = live ? ws.ml[slot(k) * 2 * MLA_M + r] : -INFINITY;
+        for (int k = part; k < pieces; k += 4) sw[k * MLA_M + r] = live ? ml[slot(k) * MLA_STATS] : -INFINITY;
         __syncthreads();
         float m = -INFINITY;
 #pragma unroll 8
@@ -990,7 +995,7 @@ __global__ void __launch_bounds__(MJ_THREADS, 2) k_mla_join(MoeKvDev kv, MlaSeqA
         for (int k = part; k < pieces; k += 4) {
             const float f = ex2(sw[k * MLA_M + r] - m0);
             sw[k * MLA_M + r] = f;
-            if (live) l = fmaf(f, ws.ml[slot(k) * 2 * MLA_M + MLA_M + r], l);
+            if (live) l = fmaf(f, ml[slot(k) * MLA_STATS + MLA_M], l);
         }
         sl[part][r] = l;
         __syncthreads();
@@ -1068,7 +1073,7 @@ int mla_pairs(int sms) { return sms / 2 < 1 ? 1 : sms / 2 > MLA_PAIRS ? MLA_PAIR
 
 size_t moe_mla_ws_bytes(int latent, int sms) {
     const int pairs = mla_pairs(sms);
-    return ((size_t)pairs * sizeof(MlaWs::Tail) + 255) / 256 * 256 + (size_t)pairs * 2 * (2 + latent) * MLA_M * sizeof(float);
+    return ((size_t)pairs * sizeof(MlaWs::Tail) + 255) / 256 * 256 + (size_t)pairs * 2 * (MLA_STATS + latent * MLA_M) * sizeof(float);
 }
 
 int moe_launch_mla(const MoeKvDev &kv, const MoeKvBatchDev &b, const MoeMlaQuery &q, void *ws, int sms, int *error,

@@ -1,0 +1,74 @@
+"""GPU: absorbed attention where a CTA pair walks over several tiles of a unit,
+so that the running reference of the softmax is raised inside a piece, and the
+pieces that pairs leave of one unit are joined: against the plain 64-bit form
+of tests/mla_ref.py."""
+import numpy as np
+import pytest
+
+import mla_ref as R
+from test_gpu_mla import Paged, m, run_attend  # noqa: F401  (m: the context fixture)
+
+pytestmark = pytest.mark.gpu
+TILE, RAISE = 64, 8.0   # cache rows of a tile; log2 by which scores may pass the reference
+LN2 = float(np.log(2.0))
+
+
+def pairs():
+    import torch
+    return torch.cuda.get_device_properties(0).multi_processor_count // 2
+
+
+def tiles_per_pair(lens, heads):
+    return sum(-(-n * heads // 128) * -(-(c + n) // TILE) for c, n in lens) / pairs()
+
+
+def bounds(want, wl, A, S, t, tiles):
+    """R.attend_bounds, whose 2^-20 of A stands for few tiles: the output's sums of a piece take 4 steps a tile, each
+    cut to fp32 at most once, the join one more per piece; sums of weights the same."""
+    tol, tl = R.attend_bounds(want, wl, A, S, t)
+    steps = (4 * tiles + pairs()) * 2.0 ** -23
+    return tol + steps * A, tl + steps
+
+
+def check(g, q, scale, out, lse, tiles):
+    t = R.kind(g.fmt)
+    qv = R.rounded(q, t)
+    for b, (c, n) in enumerate(g.lens):
+        s = slice(g.start[b], g.start[b + 1])
+        kv = R.unpack(g.host[g.rows(b, 0, c + n)], g.latent, g.fmt)
+        vis = np.concatenate([np.ones((n, c), bool), np.tril(np.ones((n, n), bool))], 1)
+        want, wl, A, S = R.attend(qv[s], kv, vis, scale, g.latent)
+        tol, tl = bounds(want, wl, A, S, t, tiles)
+        bad = ~(np.abs(out[s] - want) <= tol)
+        assert not bad.any(), (b, bad.sum(), np.argwhere(bad)[:4], out[s][bad][:4], want[bad][:4], tol[bad][:4])
+        assert np.all(np.abs(lse[s] - wl) <= tl), (b, np.max(np.abs(lse[s] - wl) - tl))
+
+
+@pytest.mark.parametrize("fmt", R.FORMATS)
+@pytest.mark.parametrize("latent", [512, 128])
+def test_halves_whose_references_part(m, cuda_lib, fmt, latent):  # noqa: F811
+    """The two CTAs of a pair sum a score's halves in different orders.  Here the halves are large and cancel, so the
+    two scores differ in their last bits; one row of a piece lies at the reference + 8 log2 up to those bits, so
+    that often one of the CTAs raises its reference there and the other does not."""
+    n_rows = 9 * pairs() * TILE - 40
+    g = Paged(cuda_lib, [(n_rows - 1, 1)], fmt, latent, 64)
+    assert tiles_per_pair(g.lens, 128) > 8
+    rng = np.random.default_rng(latent)
+    half = np.abs(rng.standard_normal((n_rows, latent // 2))) * 4
+    # scores in log2: the reference's row of each tile 0, the others far below it, one row of every ninth tile + 8
+    target = np.full(n_rows, -10.0)
+    target[::TILE] = 0.0
+    target[4 * TILE + 5::9 * TILE] = RAISE
+    rope = np.zeros((n_rows, 64))
+    rope[:, 0] = target
+    # page by page: the rows are many
+    g.host[g.rows(0, 0, n_rows)] = R.pack(np.concatenate([half, half], 1).astype(np.float32), rope.astype(np.float32), fmt)
+    g.upload()
+    q = np.zeros((1, 128, latent + 64))
+    side = np.repeat(np.abs(rng.standard_normal((4, latent // 2))), 32, 0)   # a warp's 32 rows alike
+    q[0, :, :latent // 2], q[0, :, latent // 2:latent] = side, -side
+    q[0, :, latent] = 1.0
+    out, lse = run_attend(m, g, q, LN2, R.kind(fmt))
+    check(g, q, LN2, out, lse, 10)
+    # rows hold the same values in both halves, so both halves of the output are the same up to their errors
+    assert np.allclose(out[..., :latent // 2], out[..., latent // 2:], rtol=0.1)
