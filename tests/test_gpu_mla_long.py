@@ -72,3 +72,33 @@ def test_halves_whose_references_part(m, cuda_lib, fmt, latent):  # noqa: F811
     check(g, q, LN2, out, lse, 10)
     # rows hold the same values in both halves, so both halves of the output are the same up to their errors
     assert np.allclose(out[..., :latent // 2], out[..., latent // 2:], rtol=0.1)
+
+
+@pytest.mark.parametrize("fmt", R.FORMATS)
+@pytest.mark.parametrize("shape", ["cut", "whole", "both"])
+def test_reference_raised_inside_a_piece(m, cuda_lib, fmt, shape):  # noqa: F811
+    """Scores that climb by more than 8 log2 from tile to tile inside a piece, fall back, and climb by less: units cut
+    into pieces of many tiles, whole units of several tiles, and both at once."""
+    p = pairs()
+    lens = {"cut": [(8 * p * TILE + 17, 1)], "whole": [(6 * TILE - 1 - (b % 3), 1) for b in range(2 * p)],
+            "both": [(5 * TILE + 3, 2)] * p + [(2 * p * TILE, 1)]}[shape]
+    heads = 128
+    assert tiles_per_pair(lens, heads) > 7
+    g = Paged(cuda_lib, lens, fmt, 128, 64, seed=1)
+    rng = np.random.default_rng(len(lens))
+    # the climb inside any 3 tiles passes 8 log2 for some heads (head h turns the climb by its own factor)
+    level = np.array([0.0, 6.0, 20.0, 3.0, 33.0, 34.0, -5.0, 60.0])
+    for b, (c, n) in enumerate(lens):
+        r = c + n
+        lat = rng.standard_normal((r, 128)).astype(np.float32) * 0.25
+        rope = np.zeros((r, 64), np.float32)
+        rope[:, 0] = level[(np.arange(r) // TILE + b) % len(level)]
+        rope[:, 1] = 0.5 * rng.standard_normal(r)
+        g.host[g.rows(b, 0, r)] = R.pack(lat, rope, fmt)
+    g.upload()
+    q = rng.standard_normal((g.T, heads, 192)) * 0.25
+    q[..., 128:] = 0
+    q[..., 128] = np.linspace(-1, 1, heads)
+    q[..., 129] = 1.0
+    out, lse = run_attend(m, g, q, LN2, R.kind(fmt))
+    check(g, q, LN2, out, lse, 10)
