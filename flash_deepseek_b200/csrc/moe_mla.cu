@@ -55,6 +55,13 @@ constexpr int MLA_SB = 3;                   // tiles of ring B
 constexpr int MLA_TM_S = 256, MLA_TM_P = 32, MLA_TM_Q = 384;
 constexpr int MLA_XW = 8;                   // warps that expand the 8-bit formats (4: 667 us where 8 take 626)
 constexpr float MLA_RAISE = 8.0f;           // log2: how far scores may pass the reference before it is raised
+// log2 of the weight of a score at the reference.  fp16 weights are normal from 2^-14 and zero below 2^-25, so they are
+// put as high as 2^(lift + MLA_RAISE) = 2^15 allows: full precision down to 2^-21 of the reference's weight, and an error
+// of at most 2^-32 of it below.  (Lifted by 0, rows 17 nats below the reference weighed twice too much or nothing: 10^5
+// of them behind one strong row are a part of the result that shows.)  bf16 has fp32's exponents and needs none.  Nor do
+// scores from 2^20 on, whose own rounding is 2^-4 and more: there the room up to fp16's 2^16 is for that.
+template <bool BF16>
+__device__ __forceinline__ float mla_lift(float score) { return !BF16 && fabsf(score) < 1048576.0f ? 7.0f : 0.0f; }
 
 // Tensor memory left for query chunks of 32 columns (64 values) each: all of
 // them for up to 256 latent values, 6 of 7 for 384, 4 of 9 for 512.
@@ -579,7 +586,7 @@ struct MlaKernel {
             const int token = live ? row / (uint32_t)q.n_heads : 0;
             const int tile0 = g.tile0, tile1 = g.tile1, ctx = s.ctx;
             load_query(r, s, (uint32_t)g.block * MLA_M);
-            float ref = -INFINITY, l = 0.0f;
+            float ref = -INFINITY, l = 0.0f;   // ref: the score whose weight is 1
             for (int t = tile0; t < tile1; t++, it++) {
                 const int64_t pos0 = (int64_t)t * MLA_N;
                 ok = wait_phase(&c->s_full[it & 1], (it >> 1) & 1);
@@ -611,10 +618,10 @@ struct MlaKernel {
                     top = fmaxf(fmaxf(m0, m1), v[31]);
                 }
                 top *= c2;
-                if (t == tile0) ref = top;
-                else if (__any_sync(0xffffffffu, top > ref + MLA_RAISE)) {
-                    // raise the reference: weights stay below 2^8 of it, so fp16 and bf16 hold them
-                    const float m = fmaxf(ref, top), f = m == -INFINITY ? 1.0f : ex2(ref - m);
+                if (t == tile0) ref = top - mla_lift<BF16>(top);
+                else if (__any_sync(0xffffffffu, top > ref + (mla_lift<BF16>(ref) + MLA_RAISE))) {
+                    // raise the reference: weights stay below 2^8 of its own, so fp16 and bf16 hold them
+                    const float m = fmaxf(ref, top - mla_lift<BF16>(top)), f = m == -INFINITY ? 1.0f : ex2(ref - m);
                     l *= f;
                     ref = m;
                     ok = output_done(it - 1);   // the output holds all tiles before this one

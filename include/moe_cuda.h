@@ -347,7 +347,8 @@ int moe_kv_read_device(moe_ctx *ctx, const moe_kv_cache *kv, const moe_kv_batch 
  * MOE_KV_FP8_F16, else bf16), strides in elements (multiples of 8), buffers
  * 16-byte aligned; d_lse fp32 [n_tokens][n_heads] or NULL.  Products of 16-bit
  * operands, sums and softmax statistics in fp32; probabilities are rounded to
- * the 16-bit type before they weight the rows.
+ * the 16-bit type before they weight the rows (half a step; in fp16, those
+ * below 2^-21 of the largest by up to 2^-32 of it).
  * Workspace: moe_mla_workspace_bytes(ctx, latent), 256-byte aligned, needs no
  * initialisation, one for each call that may run at the same time. */
 typedef struct moe_mla_query {

@@ -102,3 +102,58 @@ def test_reference_raised_inside_a_piece(m, cuda_lib, fmt, shape):  # noqa: F811
     q[..., 129] = 1.0
     out, lse = run_attend(m, g, q, LN2, R.kind(fmt))
     check(g, q, LN2, out, lse, 10)
+
+
+@pytest.mark.parametrize("fmt", R.FORMATS)
+@pytest.mark.parametrize("below", [8.0, 13.0, 16.0, 17.2, 17.35, 19.0])
+def test_a_strong_first_row_does_not_hide_the_tail(m, cuda_lib, fmt, below):  # noqa: F811
+    """One row (of value 0) takes most of the weight in front of 131,071 rows (of value 1), `below` nats lower."""
+    n_rows, latent = 131072, 128
+    g = Paged(cuda_lib, [(n_rows - 1, 1)], fmt, latent, 64, seed=2)
+    lat = np.ones((n_rows, latent), np.float32)
+    lat[0] = 0
+    rope = np.zeros((n_rows, 64), np.float32)
+    rope[0, 0] = 1
+    g.host[g.rows(0, 0, n_rows)] = R.pack(lat, rope, fmt)
+    g.upload()
+    q = np.zeros((1, 16, latent + 64))
+    q[..., latent] = np.linspace(0.9, 1.0, 16) * 64
+    scale = below / 64
+    t = R.kind(fmt)
+    out, lse = run_attend(m, g, q, scale, t)
+    # in closed form (the rows are two kinds): weights 1 and e^-s, s the strong row's score
+    s = scale * R.rounded(q, t)[0, :, latent]
+    tail = (n_rows - 1) * np.exp(-s)
+    want = tail / (1 + tail)
+    # as R.attend_bounds, and what fp16 adds: a weight of at least 2^-32 of the reference's keeps an error of at most
+    # that, for each row, where it is below fp16's normal range; then the sums' steps
+    tol, tl = bounds(want[:, None], s + np.log1p(tail), want[:, None], s, t, -(-n_rows // TILE) / pairs() + 1)
+    if t == "f16":
+        tol = tol + (n_rows * 2.0 ** -32 / (1 + tail))[:, None]
+    assert np.all(np.abs(out[0] - want[:, None]) <= tol), (out[0, :, 0], want, tol[:, 0])
+    assert np.all(np.abs(lse[0] - s - np.log1p(tail)) <= tl)
+
+
+@pytest.mark.parametrize("fmt", R.FORMATS)
+@pytest.mark.parametrize("size", [2.0 ** 18, 2.0 ** 23, 2.0 ** 25])
+def test_huge_scores_stay_finite(m, cuda_lib, fmt, size):  # noqa: F811
+    """Scores (in log2, up to twice `size`) whose own rounding is up to 4: the strongest row wins, nothing overflows."""
+    p = pairs()
+    n_rows = 8 * p * TILE
+    g = Paged(cuda_lib, [(n_rows - 1, 1)], fmt, 128, 64, seed=3)
+    rng = np.random.default_rng(1)
+    lat = rng.standard_normal((n_rows, 128)).astype(np.float32)
+    rope = np.zeros((n_rows, 64), np.float32)
+    rope[:, 0] = rng.uniform(0.5, 1.0, n_rows)
+    rope[n_rows // 3 + 7, 0] = 2.0
+    g.host[g.rows(0, 0, n_rows)] = R.pack(lat, rope, fmt)
+    g.upload()
+    q = np.zeros((1, 128, 192))
+    q[..., 128] = np.linspace(0.5, 1.0, 128)
+    scale = size * LN2
+    out, lse = run_attend(m, g, q, scale, R.kind(fmt))
+    row = R.unpack(g.host[g.rows(0, n_rows // 3 + 7, n_rows // 3 + 8)], 128, fmt)[0, :128]
+    want = np.broadcast_to(row, (128, 128))
+    s = scale * R.rounded(q, R.kind(fmt))[0, :, 128] * 2.0
+    assert np.all(np.abs(out[0] - want) <= 2 * R.U[R.kind(fmt)] * np.abs(want) * 1.01)
+    assert np.all(np.abs(lse[0] - s) <= 2.0 ** -20 * s)
