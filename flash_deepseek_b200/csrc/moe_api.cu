@@ -1667,6 +1667,7 @@ int moe_mla_attention_device(moe_ctx *c, const moe_kv_cache *kv, const moe_kv_ba
     if (!c) return MOE_ERR_ARG;
     const char *bad = kv_bad_cache(kv, b);
     if (!bad) bad = kv_bad_query(kv, b, q, ws, ws_bytes, moe_mla_ws_bytes(kv->latent, c->sms));
+    if (!bad) bad = kv_bad_in_place(b, q);
     if (bad) return fail(c, MOE_ERR_ARG, "moe_mla_attention_device: %s", bad);
     if (b->n_tokens == 0 || b->n_seqs == 0) return MOE_OK;
     const MoeMlaQuery dq{q->q_latent, q->q_rope, q->q_latent_token_stride, q->q_latent_head_stride,

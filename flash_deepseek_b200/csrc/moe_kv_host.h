@@ -132,3 +132,11 @@ inline const char *kv_bad_query(const moe_kv_cache *kv, const moe_kv_batch *b, c
     if (!ws || kv_off(ws, 256) || ws_bytes < ws_need) return "workspace null, not 256-byte aligned or too small";
     return nullptr;
 }
+
+// The attention's output may not be one of its query's buffers: the CTAs that share a block of query rows, and the pairs
+// that share a unit, read the query at their own times, while others store results.
+inline const char *kv_bad_in_place(const moe_kv_batch *b, const moe_mla_query *q) {
+    if (b->n_tokens == 0 || b->n_seqs == 0) return nullptr;
+    if (q->out == q->q_latent || q->out == q->q_rope) return "output and query are the same buffer";
+    return nullptr;
+}

@@ -339,16 +339,16 @@ int moe_kv_read_device(moe_ctx *ctx, const moe_kv_cache *kv, const moe_kv_batch 
  * included.  d_tree NULL: a causal chain (j <= its own number).  Rows that a
  * token does not see never touch its output, whatever they hold; a visible
  * row with a NaN makes it NaN (with an infinity: NaN or what IEEE arithmetic
- * leaves).  A token that sees nothing gets
- * out = 0 and lse = -infinity.  Rows of the call that tree_words does not
- * reach are not seen.
+ * leaves).  A token that sees nothing gets out = 0 and lse = -infinity.  Rows
+ * of the call that tree_words does not reach are not seen.
  * q_latent [token][head][latent], q_rope [token][head][64], out
  * [token][head][latent] in the cache's 16-bit type (fp16 for MOE_KV_F16 and
  * MOE_KV_FP8_F16, else bf16), strides in elements (multiples of 8), buffers
- * 16-byte aligned; d_lse fp32 [n_tokens][n_heads] or NULL.  Products of 16-bit
- * operands, sums and softmax statistics in fp32; probabilities are rounded to
- * the 16-bit type before they weight the rows (half a step; in fp16, those
- * below 2^-21 of the largest by up to 2^-32 of it).
+ * 16-byte aligned, out apart from the query's buffers; d_lse fp32
+ * [n_tokens][n_heads] or NULL.  Products of 16-bit operands, sums and softmax
+ * statistics in fp32; probabilities are rounded to the 16-bit type before they
+ * weight the rows (half a step; in fp16, those below 2^-21 of the largest by
+ * up to 2^-32 of it).
  * Workspace: moe_mla_workspace_bytes(ctx, latent), 256-byte aligned, needs no
  * initialisation, one for each call that may run at the same time. */
 typedef struct moe_mla_query {

@@ -75,3 +75,16 @@ def test_pages_that_sequences_share(m, cuda_lib, fmt):  # noqa: F811
     q = np.random.default_rng(11).standard_normal((g.T, 20, 320))
     out, lse = run_attend(m, g, q, 0.1, R.kind(fmt))
     check_attend(g, q, 0.1, out, lse, chain(lens))
+
+
+def test_output_in_the_querys_place_is_refused(m, cuda_lib):  # noqa: F811
+    import torch
+    F = cuda_lib
+    g = Paged(F, [(8, 1)], R.BF16, 128, 8)
+    ws = torch.empty(m.mla_workspace_bytes(128), dtype=torch.uint8, device="cuda")
+    a, b = (torch.zeros(1, 2, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    before = m.kernel_launches
+    for q_latent, q_rope in ((a, b), (b, a)):
+        with pytest.raises(F.MoeError, match="same buffer"):
+            m.mla_attention_device(g.kv, g.batch(), q_latent, (256, 128), q_rope, (256, 128), 2, 0.1, a, (256, 128), ws, ws.numel())
+    assert m.kernel_launches == before

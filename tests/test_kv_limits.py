@@ -1,4 +1,4 @@
-"""CPU: the work division of the MLA attention at the limits of its numbers."""
+"""CPU: the work division of the MLA attention at the limits of its numbers, and buffers that it must not share."""
 import os
 import re
 import subprocess
@@ -20,3 +20,14 @@ def test_the_search_for_a_share_is_bounded():
     """The thread that finds the share's first sequence looks at its own stretch of sequences only."""
     text = open(os.path.join(ROOT, "flash_deepseek_b200", "csrc", "moe_mla.cu")).read()
     assert "for (;; b++)" not in text and re.search(r"for \(; b < b1 - 1; b\+\+\)", text)
+
+
+def test_output_in_the_querys_place_is_refused(tmp_path):
+    exe = str(tmp_path / "kv_in_place")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", os.path.join(ROOT, "tests", "kv_in_place.cc"), "-o", exe],
+                   check=True)
+    said = subprocess.run([exe], capture_output=True, text=True, timeout=60, check=True).stdout.splitlines()
+    got = dict(line.split(": ", 1) for line in said)
+    assert len(got) == 5 and {k for k, v in got.items() if v != "ok"} == {"latent", "rope"}
+    api = open(os.path.join(ROOT, "flash_deepseek_b200", "csrc", "moe_api.cu")).read()
+    assert "kv_bad_in_place(b, q)" in api[api.index("int moe_mla_attention_device"):]
