@@ -241,14 +241,16 @@ uint32_t moe_rng_advance(uint32_t state, int n);
  * latent + 64 values that the token sees, and the output is the weighted mean
  * of the rows' latent parts, so one cached row serves all heads.  All entry
  * points take device pointers and are asynchronous on `stream` (NULL = the
- * context's stream); none allocates, waits or keeps state between calls, so
- * they can be captured into CUDA graphs, and calls on different streams may
- * overlap as long as they do not write the same buffers (moe_mla_attention:
- * the same workspace).  Arguments that live on the device (sequence bounds,
- * page tables) are checked by the kernels: a row that lies outside its page
- * table, or whose page is out of range, is skipped (moe_kv_write), reads as
- * zeros (moe_kv_read) or is seen by nobody (moe_mla_attention, which also skips
- * a sequence whose bounds pass the call's rows or whose context is negative),
+ * context's stream); none allocates, waits or keeps anything on the device
+ * between calls (the host keeps the frequency table of the last rotary
+ * configuration, copied into each call), so they can be captured into CUDA
+ * graphs, and calls on different streams may overlap as long as they do not
+ * write the same buffers (moe_mla_attention: the same workspace).  Arguments
+ * that live on the device (sequence bounds, page tables) are checked by the
+ * kernels: a row that lies outside its page table, or whose page is out of
+ * range, is skipped (moe_kv_write), reads as zeros (moe_kv_read) or is seen by
+ * nobody (moe_mla_attention, which also skips a sequence whose bounds pass the
+ * call's rows or whose context is negative, and cuts one at 2^31 - 65 rows),
  * and moe_check_error() reports MOE_ERR_ARG. */
 #define MOE_KV_ROPE 64      /* rotary values of a cache row (QK_ROPE_HEAD_DIM) */
 #define MOE_KV_F16 1        /* rows of (latent + 64) fp16 */
@@ -256,7 +258,11 @@ uint32_t moe_rng_advance(uint32_t state, int n);
 /* 8-bit rows: `latent` e4m3 codes, 64 rotary values of fp16 / bf16, latent/32
  * scale bytes (127 + k: the 32 codes of a group stand for code * 2^k, k the
  * least with amax <= 448 * 2^k, kept in [-15, 7]; larger values saturate, and
- * a group with an infinity or a NaN reads as NaN), padded to 16 bytes. */
+ * a group with an infinity or a NaN has scale byte 255 and reads as NaN),
+ * padded to 16 bytes.  Rows that other code fills keep to what moe_kv_write
+ * makes: scale bytes 112 .. 134, codes 0x7F and 0xFF (NaN) only in groups of
+ * scale byte 255.  moe_kv_read and moe_mla_attention may take others for
+ * different values. */
 #define MOE_KV_FP8_F16 101
 #define MOE_KV_FP8_BF16 130
 
@@ -287,7 +293,11 @@ typedef struct moe_kv_batch {
  * dim / 2 turns by theta^(-2 i / dim) radians per position; with scale > 1
  * (YaRN) the frequencies whose wavelength exceeds orig_ctx / beta_slow are
  * divided by scale, those below orig_ctx / beta_fast kept, a linear ramp over
- * the pair index between.  cos and sin are multiplied by mscale. */
+ * the pair index between.  As in the reference the ramp begins and ends at
+ * whole pairs, rounded outwards and kept within 0 .. dim / 2 - 1: where
+ * orig_ctx / beta_slow exceeds every wavelength (about 47,000 positions for
+ * theta 10000, dim 64), the last pair is still divided by the whole scale.
+ * cos and sin are multiplied by mscale. */
 typedef struct moe_rope_config {
     int dim;          /* rotated values, even, 2 .. 256 */
     int half_layout;  /* 0: pairs (2i, 2i + 1); 1: pairs (i, i + dim / 2) */
