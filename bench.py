@@ -156,6 +156,10 @@ class Clocks:
 
 
 # ----------------------------------------------------------------- CPU path
+class NoReference(Exception):
+    """The reference's CPU path is neither built nor buildable here."""
+
+
 def cpu_reference(workload: str, steps: int, warmup: int, seconds: float = 20.0):
     """The reference's CPU expert path (oracle/_ref: quant.c + route() of the
     reference, plain-C dots in place of Accelerate) on sampled tokens."""
@@ -165,6 +169,8 @@ def cpu_reference(workload: str, steps: int, warmup: int, seconds: float = 20.0)
     threads = len(os.sched_getaffinity(0))
     if not O.ref_available():
         O.build()
+    if not O.ref_available():
+        raise NoReference("the reference's CPU path is compiled from its sources (quant.c, infer.m), which are not here")
     R = O.ref()
     router = O.normal(0, O.stream(0, 0, O.KIND_ROUTER), E * H, 0.006, threads=threads).reshape(E, H)
     bias = O.normal(0, O.stream(0, 0, O.KIND_BIAS), E, 0.01, threads=threads)
@@ -423,7 +429,10 @@ def run_ours(args):
 
     cpu = None
     if rank == 0 and world == 1 and not args.no_cpu:
-        cpu = cpu_reference(args.workload, steps=20, warmup=1, seconds=15.0)
+        try:
+            cpu = cpu_reference(args.workload, steps=20, warmup=1, seconds=15.0)
+        except NoReference as e:
+            cpu = {"unavailable": str(e)}
 
     if rank == 0:
         line = {
@@ -872,7 +881,11 @@ def run_reference(args):
     if rank != 0:
         return
     W = WORKLOADS[args.workload]
-    cpu = cpu_reference(args.workload, steps=args.steps, warmup=args.warmup, seconds=60.0)
+    try:
+        cpu = cpu_reference(args.workload, steps=args.steps, warmup=args.warmup, seconds=60.0)
+    except NoReference as e:
+        print(json.dumps({"impl": "reference", "unavailable": str(e)}), flush=True)
+        return
     # the GPU arm's config at this world size (its per-GPU token share)
     from flash_deepseek_b200 import ep
     b_loc = ep.local_tokens(W["B"], world, 0)[1]
