@@ -1623,7 +1623,7 @@ int moe_rope_device(moe_ctx *c, const moe_rope_config *rope, const void *x, int 
         return fail(c, MOE_ERR_ARG, "moe_rope_device: %s", bad);
     if (T == 0 || n_heads == 0) return MOE_OK;
     DeviceScope ds(c->device);
-    moe_launch_rope(rope_dev(c, rope), x, x_type, xt, xh, y, y_type, yt, yh, d_pos, T, n_heads, head_dim, offset,
+    moe_launch_rope(rope_dev(c, rope), x, x_type, xt, xh, y, y_type, yt, yh, d_pos, T, n_heads, head_dim, offset, c->sms,
                     stream ? (cudaStream_t)stream : c->stream, &c->launches);
     CK(cudaGetLastError());
     return MOE_OK;
@@ -1652,7 +1652,7 @@ int moe_kv_read_device(moe_ctx *c, const moe_kv_cache *kv, const moe_kv_batch *b
     if (bad) return fail(c, MOE_ERR_ARG, "moe_kv_read_device: %s", bad);
     if (b->n_tokens == 0 || b->n_seqs == 0) return MOE_OK;
     DeviceScope ds(c->device);
-    moe_launch_kv_read(kv_dev(kv), batch_dev(b), y, type, stride, c->plan.error,
+    moe_launch_kv_read(kv_dev(kv), batch_dev(b), y, type, stride, c->sms, c->plan.error,
                        stream ? (cudaStream_t)stream : c->stream, &c->launches);
     CK(cudaGetLastError());
     return MOE_OK;

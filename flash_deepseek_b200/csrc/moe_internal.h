@@ -329,13 +329,13 @@ struct MoeMlaQuery {
 };
 void moe_launch_rope(const MoeRopeDev &rope, const void *x, int x_type, long long xt, long long xh, void *y,
                      int y_type, long long yt, long long yh, const int *pos, int n_tokens, int n_heads, int head_dim,
-                     int offset, cudaStream_t s, uint64_t *launches);
+                     int offset, int sms, cudaStream_t s, uint64_t *launches);
 // rope: nullptr keeps the rotary values as given
 void moe_launch_kv_write(const MoeKvDev &kv, const MoeKvBatchDev &b, const void *x, int type, long long stride,
                          const float *norm_w, float eps, const MoeRopeDev *rope, const int *pos, int *error,
                          cudaStream_t s, uint64_t *launches);
-void moe_launch_kv_read(const MoeKvDev &kv, const MoeKvBatchDev &b, void *y, int type, long long stride, int *error,
-                        cudaStream_t s, uint64_t *launches);
+void moe_launch_kv_read(const MoeKvDev &kv, const MoeKvBatchDev &b, void *y, int type, long long stride, int sms,
+                        int *error, cudaStream_t s, uint64_t *launches);
 size_t moe_mla_ws_bytes(int latent, int sms);
 // 0 = launched; otherwise a driver error while the tensor map was made
 int moe_launch_mla(const MoeKvDev &kv, const MoeKvBatchDev &b, const MoeMlaQuery &q, void *ws, int sms, int *error,

@@ -142,10 +142,10 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope_any(RopeArgs a, MoeRopeDev 
 // Cache rows.  One warp per row: a lane holds 8 consecutive latent values of
 // every 256 (so a group of 32 is 4 lanes, and loads and stores of a warp are
 // contiguous) and one rotary pair.  32,762 fp32 rows into 8 bits: 25 us (3.9
-// TB/s); 130,000 8-bit rows out as bf16: 42 us (5.7 TB/s).
+// TB/s); 130,000 8-bit rows out as bf16: 39 to 42 us by box (6.0 to 5.7 TB/s).
 // ---------------------------------------------------------------------------
 constexpr int KV_WARPS = 4;
-// rows of a reading warp in flight: 1 / 2 / 3 / 4 took 43.4 / 39.4 / 39.6 / 39.5 us for 130,000 8-bit rows
+// rows of a reading warp in flight: 1 / 2 / 3 / 4 took 43.4 / 39.4 / 39.6 / 39.5 us for 130,000 8-bit rows on one box
 constexpr int KV_RPW = 2;
 constexpr int KV_CHUNKS = 2;   // 256-value chunks of the widest latent part (512)
 
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32) k_kv_read(MoeKvDev kv, MoeKvBat
 }
 
 // rows of a warp: KV_RPW once that leaves every SM 16 warps, else 1 (a short call is all latency)
-int rows_per_warp(int rows) { return rows >= KV_RPW * 16 * 148 ? KV_RPW : 1; }
+int rows_per_warp(int rows, int sms) { return rows >= KV_RPW * 16 * sms ? KV_RPW : 1; }
 
 bool aligned16(const void *p, long long bytes) { return ((uintptr_t)p & 15) == 0 && (bytes & 15) == 0; }
 
@@ -332,7 +332,7 @@ void by_type(int type, F &&f) {
 
 void moe_launch_rope(const MoeRopeDev &rope, const void *x, int x_type, long long xt, long long xh, void *y,
                      int y_type, long long yt, long long yh, const int *pos, int n_tokens, int n_heads, int head_dim,
-                     int offset, cudaStream_t s, uint64_t *launches) {
+                     int offset, int sms, cudaStream_t s, uint64_t *launches) {
     if (n_tokens <= 0 || n_heads <= 0) return;
     RopeArgs a{x, y, xt, xh, yt, yh, pos, n_tokens, n_heads, head_dim, offset, x == y, 0, 1};
     const size_t xs = type_size(x_type), ys = type_size(y_type);
@@ -347,13 +347,13 @@ void moe_launch_rope(const MoeRopeDev &rope, const void *x, int x_type, long lon
     // some 8 units per thread, so that the last items end together)
     const int most = (a.units + RP_THREADS - 1) / RP_THREADS;
     a.parts = (a.units + RP_THREADS * 8 - 1) / (RP_THREADS * 8);
-    while (a.parts < most && (long long)n_tokens * a.parts < 148 * 8) a.parts++;
+    while (a.parts < most && (long long)n_tokens * a.parts < 8 * sms) a.parts++;
     const long long items = (long long)n_tokens * a.parts;
     by_type(x_type, [&](auto ti) {
         by_type(y_type, [&](auto to) {
             using TI = decltype(ti);
             using TO = decltype(to);
-            const unsigned ctas = (unsigned)(items < 148 * 8 ? items : 148 * 8);
+            const unsigned ctas = (unsigned)(items < 8 * sms ? items : 8 * sms);
             constexpr bool SAME = std::is_same<TI, TO>::value;   // in place: the same type (checked by the caller)
             if (vec && a.in_place) k_rope<TI, TO, RP_UNITS, SAME><<<ctas, RP_THREADS, 0, s>>>(a, rope);
             else if (vec) k_rope<TI, TO, RP_UNITS, false><<<ctas, RP_THREADS, 0, s>>>(a, rope);
@@ -393,11 +393,11 @@ void moe_launch_kv_write(const MoeKvDev &kv, const MoeKvBatchDev &b, const void 
     LAUNCH_COUNT(launches);
 }
 
-void moe_launch_kv_read(const MoeKvDev &kv, const MoeKvBatchDev &b, void *y, int type, long long stride, int *error,
-                        cudaStream_t s, uint64_t *launches) {
+void moe_launch_kv_read(const MoeKvDev &kv, const MoeKvBatchDev &b, void *y, int type, long long stride, int sms,
+                        int *error, cudaStream_t s, uint64_t *launches) {
     if (b.n_tokens <= 0 || b.n_seqs <= 0) return;
     const bool vec = aligned16(y, stride * type_size(type));
-    const int rpw = rows_per_warp(b.n_tokens), grid = (b.n_tokens + KV_WARPS * rpw - 1) / (KV_WARPS * rpw);
+    const int rpw = rows_per_warp(b.n_tokens, sms), grid = (b.n_tokens + KV_WARPS * rpw - 1) / (KV_WARPS * rpw);
     by_type(type, [&](auto to) {
         by_format<decltype(to)>(kv.format, [&](auto t, auto tc, auto fp8) {
             using TO = decltype(t);

@@ -93,7 +93,6 @@ struct MlaCtl {   // control block behind the tiles
     int seq0;
     uint32_t tmem;
     int used;                    // 8-bit formats: tiles whose copies the other CTA's scores are done with
-    int dead;                    // a bounded wait gave up
 };
 
 // Pieces of cut units: [pair][slot][latent][128 rows] sums, [pair][slot][half][2][128] references and sums of weights.
@@ -256,10 +255,7 @@ struct MlaKernel {
         return w;
     }
     __device__ __forceinline__ void give_up() {
-        if (lane == 0) {
-            c->dead = 1;
-            kv_error(error, KV_ERR_TIMEOUT);
-        }
+        if (lane == 0) kv_error(error, KV_ERR_TIMEOUT);
     }
     __device__ __forceinline__ long long flat(int seq, const MlaSeq &s, int64_t pos) const {
         if (pos >= s.len) return -2;   // behind the sequence: no error
@@ -326,7 +322,7 @@ struct MlaKernel {
         }
     }
 
-    // ---- 8-bit formats: 4 warps expand the chunks of this CTA's half into ring B, 4 threads per row, 16 codes of a chunk
+    // ---- 8-bit formats: 8 warps expand the chunks of this CTA's half into ring B, 4 threads per row, 16 codes of a chunk
     // each; from there they are copied into ring A of the other CTA, whose scores need them too.  So each CTA reads and
     // expands half of a row.  Codes are loaded a tile ahead, page numbers two.
     struct Cursor {   // a place in the pair's tiles
@@ -354,14 +350,15 @@ struct MlaKernel {
         return page < 0 || page >= kv.n_pages ? nullptr : kv.data + (((int64_t)page << kv.page_shift) + in_page) * kv.row_bytes;
     }
     __device__ void produce_expand() {
-        constexpr int L = 128 * NV, RT = 8 / MLA_XW;   // rows of a thread: r, and r + 32
+        constexpr int L = 128 * NV;
+        static_assert(MLA_XW * 32 == MLA_N * 4, "4 threads for each row of a tile");
         const int tid = threadIdx.x - 256, r = tid >> 2, qd = tid & 3;
         const int n = (int)(c->w1 - c->w0);
         const uint32_t sw = (uint32_t)(r & 7), at = (uint32_t)(r >> 3) * 1024 + sw * 128;
         const uint32_t lo_at = at + ((2 * qd) ^ sw) * 16, hi_at = at + ((2 * qd + 1) ^ sw) * 16;
         const int code_at = half * NV * 64 + qd * 16, scale_at = L + 2 * MOE_KV_ROPE + half * NV * 2 + (qd >> 1);
-        uint4 code[RT][NV];
-        uint32_t sb[RT][NV];
+        uint4 code[NV];
+        uint32_t sb[NV];
         auto load = [&](const uint8_t *row, int p, uint4 &v, uint32_t &b) {
             v = row ? __ldg(reinterpret_cast<const uint4 *>(row + code_at + p * 64)) : make_uint4(0, 0, 0, 0);
             b = row ? __ldg(row + scale_at + p * 2) : 127u;
@@ -369,42 +366,29 @@ struct MlaKernel {
         Cursor u{walk(), MlaSeg{}, 0, true};
         u.more = u.w.next(u.g, seq_at);
         u.t = u.g.tile0;
-        int page[RT], in_page[RT];
-        auto look = [&]() {
+        int in_page, page = page_of(u, r, in_page);
+        const uint8_t *row = row_of(page, in_page);
 #pragma unroll
-            for (int k = 0; k < RT; k++) page[k] = page_of(u, r + 32 * k, in_page[k]);
-        };
-        look();
-#pragma unroll
-        for (int k = 0; k < RT; k++) {
-            const uint8_t *row = row_of(page[k], in_page[k]);
-#pragma unroll
-            for (int p = 0; p < NV; p++) load(row, p, code[k][p], sb[k][p]);
-        }
+        for (int p = 0; p < NV; p++) load(row, p, code[p], sb[p]);
         step(u);
-        look();
+        page = page_of(u, r, in_page);
 #pragma unroll 1
         for (int i = 0; i < n; i++) {
             const int st = i % MLA_SB;
-            const uint8_t *row[RT];   // of tile i + 1
-#pragma unroll
-            for (int k = 0; k < RT; k++) row[k] = row_of(page[k], in_page[k]);
+            row = row_of(page, in_page);         // of tile i + 1
             step(u);
-            look();                   // the pages of tile i + 2
+            page = page_of(u, r, in_page);       // of tile i + 2
             if (!wait_phase(&c->empty_b[st], (i / MLA_SB + 1) & 1)) return give_up();
 #pragma unroll
             for (int p = 0; p < NV; p++) {
-#pragma unroll
-                for (int k = 0; k < RT; k++) {
-                    const uint32_t f = scale2<BF16>(sb[k][p]);
-                    const uint4 v = code[k][p];
-                    load(row[k], p, code[k][p], sb[k][p]);
-                    const uint2 a = expand4<BF16>(v.x, f), b = expand4<BF16>(v.y, f);
-                    const uint2 d = expand4<BF16>(v.z, f), e = expand4<BF16>(v.w, f);
-                    uint8_t *dst = ring_b + (st * NV + p) * MLA_CHUNK + k * 4096;   // 32 rows further
-                    *reinterpret_cast<uint4 *>(dst + lo_at) = make_uint4(a.x, a.y, b.x, b.y);
-                    *reinterpret_cast<uint4 *>(dst + hi_at) = make_uint4(d.x, d.y, e.x, e.y);
-                }
+                const uint32_t f = scale2<BF16>(sb[p]);
+                const uint4 v = code[p];
+                load(row, p, code[p], sb[p]);
+                const uint2 a = expand4<BF16>(v.x, f), b = expand4<BF16>(v.y, f);
+                const uint2 d = expand4<BF16>(v.z, f), e = expand4<BF16>(v.w, f);
+                uint8_t *dst = ring_b + (st * NV + p) * MLA_CHUNK;
+                *reinterpret_cast<uint4 *>(dst + lo_at) = make_uint4(a.x, a.y, b.x, b.y);
+                *reinterpret_cast<uint4 *>(dst + hi_at) = make_uint4(d.x, d.y, e.x, e.y);
             }
             fence_async_smem();
             __syncwarp();
@@ -851,7 +835,7 @@ __global__ void __launch_bounds__(FP8 ? 256 + 32 * MLA_XW : 256, 1)
         tc_mbar_init(&c->p_full[0], 4), tc_mbar_init(&c->p_full[1], 4);
         tc_mbar_init(&c->pv_done[0], 1), tc_mbar_init(&c->pv_done[1], 1);
         tc_mbar_init(&c->q_ready, 4), tc_mbar_init(&c->clean, 4), tc_mbar_init(&c->drain, FP8 ? 2 : 1);
-        c->dead = 0, c->used = 0;
+        c->used = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         if (FP8)
             for (int i = 0; i < NV; i++) tc_expect(&c->full_a[i], MLA_CHUNK);   // the other CTA's first chunks
@@ -936,7 +920,9 @@ constexpr int MLA_PAIRS = 256;   // CTA pairs at most
 static_assert(MLA_PAIRS <= 4 * MLA_M, "a thread of the join per pair");
 constexpr int MJ_THREADS = 4 * MLA_M;
 
-// columns col .. col + W - 1 of a thread's row over all pieces, U pieces' loads in flight
+// Columns col .. col + W - 1 of a thread's row over all pieces, U pieces' loads in flight: as many as fit 64 registers
+// without spilling.  1 x 25 joins 74 pieces of 80 rows in 19.9 us; 1 x 32 spills and takes 25.1, and so does 1 x 16 as
+// compiled here (18.9, but 13.0 instead of 12.5 for units of 2 or 3 pieces, by the spilled registers of all variants).
 template <int W, int U, typename S>
 __device__ __forceinline__ void join_columns(const float *o, const float *sw, int r, int pieces, size_t stride, S &&slot, float (&sum)[W]) {
     for (int k0 = 0; k0 < pieces; k0 += U) {
@@ -1018,8 +1004,7 @@ __global__ void __launch_bounds__(MJ_THREADS, 2) k_mla_join(MoeKvDev kv, MlaSeqA
                 const float *o = ws.o + (size_t)col * MLA_M + r;
                 if (mine >= 4) {
                     float a[4] = {};
-                    if (pieces <= 4) join_columns<4, 4>(o, sw, r, pieces, stride, slot, a);
-                    else join_columns<4, 8>(o, sw, r, pieces, stride, slot, a);
+                    join_columns<4, 8>(o, sw, r, pieces, stride, slot, a);
                     *reinterpret_cast<uint2 *>(out + col) = make_uint2(pack2<BF16>(a[0] * f, a[1] * f), pack2<BF16>(a[2] * f, a[3] * f));
                 } else if (mine == 2) {
                     float a[2] = {};
