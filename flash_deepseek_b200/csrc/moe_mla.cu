@@ -23,17 +23,20 @@
 // swizzled tile), one issues the MMAs, four hold one query row per thread
 // (softmax, output).  Order on the tensor pipe: scores of tile i + 1, then
 // the output product of tile i, so the softmax of one tile runs under the
-// products of its neighbours.  A tile's latent chunks of this CTA's half stay
+// products of its neighbours.  (Scores of tile i + 2 wait until that product
+// is done: they take the place of its weights.)  A tile's latent chunks of this CTA's half stay
 // until its output product is done (ring B, 3 tiles); the other half and the
 // rotary chunk are only scores' operands and leave chunk by chunk (ring A).
 // Work division: moe_kv_plan.h; cut units are joined by k_mla_join.
 //
 // Measured.  A tile's products take 1,984 cycles (128 x 64 scores: 32 cycles per
 // 16 values with the query in tensor memory, 48 from shared memory, whose reads
-// bound it; 128 x 256 output: 128 cycles per 16 rows); a tile takes some 2,500
-// in 16 bits and 3,200 in 8 bits, where the pair runs in lockstep.  32 sequences
-// of 8192 bf16 rows, one token of 128 heads: 112 us (2.5 TB/s, 0.65 PFLOP/s);
-// 8 trees of 13 tokens over 16,384 8-bit rows: 0.62 ms (0.7 PFLOP/s).
+// bound it; 128 x 256 output: 128 cycles per 16 rows); a tile takes some 2,900
+// (1.7 us) in 16 bits and 3,200 (1.9 us) in 8 bits, where the pair runs in
+// lockstep, and a launch 14 to 17 us beside its tiles.  With the join (10 to 23
+// us, partly under it): 32 sequences of 8192 bf16 rows, one token of 128 heads:
+// 113 to 134 us by box (2.4 to 2.1 TB/s, 0.57 to 0.48 PFLOP/s); 8 trees of 13
+// tokens over 16,384 8-bit rows: 0.65 to 0.70 ms (0.66 to 0.61 PFLOP/s).
 #include "moe_common.cuh"
 #include "moe_kv.cuh"
 #include "moe_kv_plan.h"
@@ -128,8 +131,8 @@ struct MlaSeqAt {
 
 // The warp waits for a phase (tc_wait_warp); the polling is out of line: the
 // loops of this kernel's roles share one instruction cache of some 32 KB, and
-// with everything unrolled and inlined a fifth to a third of the fetches missed
-// it, which cost more than any other stall.
+// with everything unrolled and inlined the wait for instructions cost more than
+// any other stall (8-bit rows: 0.80 against 0.64 ms).
 __device__ __noinline__ bool poll(uint64_t *b, uint32_t parity) { return tc_wait_warp(b, parity); }
 __device__ __forceinline__ bool wait_phase(uint64_t *b, uint32_t parity) {
     return __all_sync(0xffffffffu, tc_test(b, parity)) || poll(b, parity);
