@@ -24,9 +24,10 @@
 // (softmax, output).  Order on the tensor pipe: scores of tile i + 1, then
 // the output product of tile i, so the softmax of one tile runs under the
 // products of its neighbours.  (Scores of tile i + 2 wait until that product
-// is done: they take the place of its weights.)  A tile's latent chunks of this CTA's half stay
-// until its output product is done (ring B, 3 tiles); the other half and the
-// rotary chunk are only scores' operands and leave chunk by chunk (ring A).
+// is done: they take the place of its weights.)  A tile's latent chunks of this
+// CTA's half stay until its output product is done (ring B, 3 tiles); the other
+// half and the rotary chunk are only scores' operands and leave chunk by chunk
+// (ring A).
 // Work division: moe_kv_plan.h; cut units are joined by k_mla_join.
 //
 // Measured.  A tile's products take 1,984 cycles (128 x 64 scores: 32 cycles per
@@ -65,6 +66,12 @@ constexpr float MLA_RAISE = 8.0f;           // log2: how far scores may pass the
 // scores from 2^20 on, whose own rounding is 2^-4 and more: there the room up to fp16's 2^16 is for that.
 template <bool BF16>
 __device__ __forceinline__ float mla_lift(float score) { return !BF16 && fabsf(score) < 1048576.0f ? 7.0f : 0.0f; }
+
+// Log of the sum of exponentials, from the reference and the sum of weights relative to it: added in log2, where a lift
+// cancels exactly
+__device__ __forceinline__ float mla_lse(float ref, float l) {
+    return l == 0.0f ? -INFINITY : (ref + log2f(l)) * 0.69314718055994531f;
+}
 
 // Tensor memory left for query chunks of 32 columns (64 values) each: all of
 // them for up to 256 latent values, 6 of 7 for 384, 4 of 9 for 512.
@@ -794,7 +801,7 @@ struct MlaKernel {
             __syncwarp();
         }
         if (live && half == 0 && q.lse)
-            q.lse[token * q.n_heads + head] = l == 0.0f ? -INFINITY : ref * 0.69314718055994531f + logf(l);
+            q.lse[token * q.n_heads + head] = mla_lse(ref, l);
     }
 
     __device__ __forceinline__ void store_piece(uint32_t tmem, bool begins, bool live, int r, float ref, float l) {
@@ -923,9 +930,9 @@ constexpr int MLA_PAIRS = 256;   // CTA pairs at most
 static_assert(MLA_PAIRS <= 4 * MLA_M, "a thread of the join per pair");
 constexpr int MJ_THREADS = 4 * MLA_M;
 
-// Columns col .. col + W - 1 of a thread's row over all pieces, U pieces' loads in flight: as many as fit 64 registers
-// without spilling.  1 x 25 joins 74 pieces of 80 rows in 19.9 us; 1 x 32 spills and takes 25.1, and so does 1 x 16 as
-// compiled here (18.9, but 13.0 instead of 12.5 for units of 2 or 3 pieces, by the spilled registers of all variants).
+// Columns col .. col + W - 1 of a thread's row over all pieces, U pieces' loads in flight: as many as the compiler fits
+// into 64 registers for all three W without spilling.  1 x 25 joins 74 pieces of 80 rows in 19.9 us; 1 x 32 spills and
+// takes 25.1; 1 x 16 takes 18.9 but makes it spill elsewhere (units of 2 or 3 pieces: 13.0 instead of 12.5).
 template <int W, int U, typename S>
 __device__ __forceinline__ void join_columns(const float *o, const float *sw, int r, int pieces, size_t stride, S &&slot, float (&sum)[W]) {
     for (int k0 = 0; k0 < pieces; k0 += U) {
@@ -1020,7 +1027,7 @@ __global__ void __launch_bounds__(MJ_THREADS, 2) k_mla_join(MoeKvDev kv, MlaSeqA
                 }
             }
             if (col0 == 0 && part == 0 && q.lse)
-                q.lse[token * q.n_heads + head] = l == 0.0f ? -INFINITY : m * 0.69314718055994531f + logf(l);
+                q.lse[token * q.n_heads + head] = mla_lse(m, l);
         }
     }
 }

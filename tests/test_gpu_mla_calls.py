@@ -88,3 +88,16 @@ def test_output_in_the_querys_place_is_refused(m, cuda_lib):  # noqa: F811
         with pytest.raises(F.MoeError, match="same buffer"):
             m.mla_attention_device(g.kv, g.batch(), q_latent, (256, 128), q_rope, (256, 128), 2, 0.1, a, (256, 128), ws, ws.numel())
     assert m.kernel_launches == before
+
+
+@pytest.mark.parametrize("fmt", R.FORMATS)
+def test_lse_of_a_few_equal_scores(m, cuda_lib, fmt):  # noqa: F811
+    """Scores of zero over 1 to 300 rows: lse = log n, within a step or two of fp32 (log2 of n: 1 ulp, one addition, one
+    product by a rounded ln 2; absolute 2^-22 where the reference's own size cancels)."""
+    lens = [(0, 1), (1, 1), (2, 1), (63, 1), (299, 1)]
+    g = Paged(cuda_lib, lens, fmt, 128, 16, seed=12)
+    fill(g, 12)
+    out, lse = run_attend(m, g, np.zeros((g.T, 3, 192)), 0.5, R.kind(fmt))
+    want = np.log([c + n for c, n in lens])[:, None]
+    assert np.all(np.abs(lse - want) <= 2.0 ** -22 * (1 + want)), lse - want
+    check_attend(g, np.zeros((g.T, 3, 192)), 0.5, out, lse, chain(lens))
