@@ -932,7 +932,8 @@ constexpr int MJ_THREADS = 4 * MLA_M;
 
 // Columns col .. col + W - 1 of a thread's row over all pieces, U pieces' loads in flight: as many as the compiler fits
 // into 64 registers for all three W without spilling.  1 x 25 joins 74 pieces of 80 rows in 19.9 us; 1 x 32 spills and
-// takes 25.1; 1 x 16 takes 18.9 but makes it spill elsewhere (units of 2 or 3 pieces: 13.0 instead of 12.5).
+// takes 25.1; 1 x 16 takes 18.9 but makes it spill elsewhere (units of 2 or 3 pieces: 13.0 instead of 12.5).  4 x 4 for
+// up to 4 pieces: half of 4 x 8's loads would be idle (32 sequences of 8192 rows: 113.1 against 114.5 us a call).
 template <int W, int U, typename S>
 __device__ __forceinline__ void join_columns(const float *o, const float *sw, int r, int pieces, size_t stride, S &&slot, float (&sum)[W]) {
     for (int k0 = 0; k0 < pieces; k0 += U) {
@@ -1014,7 +1015,8 @@ __global__ void __launch_bounds__(MJ_THREADS, 2) k_mla_join(MoeKvDev kv, MlaSeqA
                 const float *o = ws.o + (size_t)col * MLA_M + r;
                 if (mine >= 4) {
                     float a[4] = {};
-                    join_columns<4, 8>(o, sw, r, pieces, stride, slot, a);
+                    if (pieces <= 4) join_columns<4, 4>(o, sw, r, pieces, stride, slot, a);
+                    else join_columns<4, 8>(o, sw, r, pieces, stride, slot, a);
                     *reinterpret_cast<uint2 *>(out + col) = make_uint2(pack2<BF16>(a[0] * f, a[1] * f), pack2<BF16>(a[2] * f, a[3] * f));
                 } else if (mine == 2) {
                     float a[2] = {};
