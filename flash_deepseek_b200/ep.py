@@ -63,8 +63,9 @@ class PeerWatch:
     Every rank calls `beat(step)` before it launches step `step` and
     `wait(step)` before the launch: `wait` returns once every rank has beaten
     `step`, or raises PeerLost naming the ranks that have not within
-    `timeout` seconds (or that called `leave()`).  Because the check sits
-    before this rank's launches, none of its kernels or exchanges of that
+    `timeout` seconds (or that called `leave()` before they beat it: a rank
+    that left after its beat of a step has arrived at that step, and is
+    missed at the next).  Because the check sits before this rank's launches, none of its kernels or exchanges of that
     step are in flight when the failure is seen, and the context can be
     destroyed at once.  `store` is a torch.distributed key-value store
     (TCPStore, FileStore or a process group's store).  The reference runs one
@@ -74,16 +75,19 @@ class PeerWatch:
         if world < 1 or not 0 <= rank < world:
             raise ValueError(f"bad rank/world {rank}/{world}")
         self.store, self.rank, self.world, self.timeout, self.prefix = store, rank, world, timeout, prefix
+        self.last = None   # step of this rank's last beat
 
     def _key(self, r: int) -> str:
         return f"{self.prefix}/{r}"
 
     def beat(self, step: int) -> None:
-        self.store.set(self._key(self.rank), str(int(step)))
+        self.last = int(step)
+        self.store.set(self._key(self.rank), str(self.last))
 
     def leave(self) -> None:
-        """A clean exit: the peers' next wait fails at once instead of timing out."""
-        self.store.set(self._key(self.rank), "-1")
+        """A clean exit: the peers' wait for a step that this rank has not beaten
+        fails at once instead of timing out."""
+        self.store.set(self._key(self.rank), "left" if self.last is None else f"left {self.last}")
 
     def wait(self, step: int) -> None:
         import time
@@ -93,11 +97,12 @@ class PeerWatch:
             left, still = [], []
             for r in pending:
                 k = self._key(r)
-                v = int(self.store.get(k)) if self.store.check([k]) else None
-                if v == -1:
-                    left.append(r)
-                elif v is None or v < step:
-                    still.append(r)
+                v = self.store.get(k) if self.store.check([k]) else b""
+                words = (v.decode() if isinstance(v, bytes) else v).split()
+                gone = words[:1] == ["left"]
+                if words[gone:] and int(words[-1]) >= step:
+                    continue
+                (left if gone else still).append(r)
             if left:
                 raise PeerLost(step, sorted(left + still), left)
             if not still:
